@@ -155,6 +155,22 @@ int pb_copy_peer(pb_ctx* ctx, int dst_dev, void* dst, int src_dev, const void* s
                  int stream_dev, int stream);
 int pb_stream_wait(pb_ctx* ctx, int waiter, int waiter_stream, int signal, int signal_stream);
 
+/* Device memory and streams of other libraries in the same process.
+ * pb_pointer_check returns PB_OK when [ptr, ptr + bytes) starts and ends in
+ * device (or managed) memory of device index `dev`, and PB_ERR_INVALID when it
+ * does not: such memory may be passed wherever an entry point takes a device
+ * pointer, if it is aligned as that entry point asks (pb_alloc gives 256
+ * bytes; 16 is enough for every one).  It is not freed by this library.
+ * pb_stream_join orders this library's stream and `stream`, a cudaStream_t of
+ * the same device (NULL: the legacy default stream): with `direction`
+ * PB_JOIN_WAIT the library's stream waits for the work queued so far on
+ * `stream`, with PB_JOIN_SIGNAL the other way round.  Neither waits on the host;
+ * PB_ERR_UNSUPPORTED while either stream is being captured.  No counterpart in
+ * the reference. */
+enum { PB_JOIN_WAIT = 0, PB_JOIN_SIGNAL = 1 };
+int pb_pointer_check(pb_ctx* ctx, int dev, const void* ptr, size_t bytes);
+int pb_stream_join(pb_ctx* ctx, int dev, void* stream, int direction);
+
 /* CUDA graphs of hot-path calls.  pb_capture_begin starts a (relaxed) capture
  * of the device stream; the entry points called until pb_capture_end are
  * recorded, not run, and pb_capture_end returns an instantiated graph that

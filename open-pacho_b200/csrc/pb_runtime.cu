@@ -573,6 +573,56 @@ int pb_stream_wait(pb_ctx* ctx, int waiter, int waiter_stream, int signal, int s
   return PB_OK;
 }
 
+int pb_pointer_check(pb_ctx* ctx, int dev, const void* ptr, size_t bytes) {
+  if (!ctx) PB_FAIL(PB_ERR_INVALID, "null context");
+  if (!ptr) PB_FAIL(PB_ERR_INVALID, "null pointer");
+  std::lock_guard<std::recursive_mutex> g(ctx->mu);
+  Device* d;
+  PB_CHECK(enter(ctx, dev, &d));
+  const char* ends[2] = {static_cast<const char*>(ptr), static_cast<const char*>(ptr) + (bytes ? bytes - 1 : 0)};
+  for (const char* p : ends) {
+    cudaPointerAttributes at = {};
+    const cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      PB_FAIL(PB_ERR_INVALID, "%p is no device pointer: %s", (const void*)p, cudaGetErrorString(e));
+    }
+    if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged)
+      PB_FAIL(PB_ERR_INVALID, "%p is not device memory", (const void*)p);
+    if (at.device != d->ordinal)
+      PB_FAIL(PB_ERR_INVALID, "%p is memory of device %d, not of device %d", (const void*)p, at.device, d->ordinal);
+  }
+  return PB_OK;
+}
+
+int pb_stream_join(pb_ctx* ctx, int dev, void* stream, int direction) {
+  if (!ctx) PB_FAIL(PB_ERR_INVALID, "null context");
+  if (direction != PB_JOIN_WAIT && direction != PB_JOIN_SIGNAL)
+    PB_FAIL(PB_ERR_INVALID, "unknown join direction %d", direction);
+  std::lock_guard<std::recursive_mutex> g(ctx->mu);
+  Device* d;
+  PB_CHECK(enter(ctx, dev, &d));
+  if (d->capturing) PB_FAIL(PB_ERR_UNSUPPORTED, "%s cannot run during stream capture", __func__);
+  // The handle 0x1 names the legacy default stream whatever the default-stream mode.
+  cudaStream_t other = stream ? static_cast<cudaStream_t>(stream) : cudaStreamLegacy;
+  if (other == d->stream) return PB_OK;
+  // Joining a stream that is being captured would pull this library's stream
+  // into that graph without its knowing.
+  cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(other, &state);
+  if (e == cudaErrorStreamCaptureImplicit || state != cudaStreamCaptureStatusNone) {
+    cudaGetLastError();  // the next launch must not report this refusal
+    PB_FAIL(PB_ERR_UNSUPPORTED, "pb_stream_join with a stream that is being captured");
+  }
+  if (e == cudaSuccess) e = cudaEventRecord(d->order_ev, direction == PB_JOIN_WAIT ? other : d->stream);
+  if (e == cudaSuccess) e = cudaStreamWaitEvent(direction == PB_JOIN_WAIT ? d->stream : other, d->order_ev, 0);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    PB_FAIL(PB_ERR_CUDA, "pb_stream_join failed: %s", cudaGetErrorString(e));
+  }
+  return PB_OK;
+}
+
 int pb_copy_peer(pb_ctx* ctx, int dst_dev, void* dst, int src_dev, const void* src, size_t bytes,
                  int stream_dev, int stream) {
   if (!ctx) PB_FAIL(PB_ERR_INVALID, "null context");

@@ -36,6 +36,9 @@ PB_GEMM_TF32X3_PRESPLIT = 4
 PB_GEMM_TF32X3_FUSED = 5
 PB_GEMM_SKINNY = 6
 
+PB_JOIN_WAIT = 0
+PB_JOIN_SIGNAL = 1
+
 # Elementwise operation codes (pacho_b200.h PB_EW_*), by the reference's
 # operation names (src/openpacho/_cuda.py:21-46).
 EW_OPS = {name: code for code, name in enumerate((
@@ -89,6 +92,8 @@ PROTOTYPES = {
     "pb_free_mapped": [_ctx, _i, C.c_void_p],
     "pb_copy_peer": [_ctx, _i, C.c_void_p, _i, C.c_void_p, _sz, _i, _i],
     "pb_stream_wait": [_ctx, _i, _i, _i, _i],
+    "pb_pointer_check": [_ctx, _i, _p, _sz],
+    "pb_stream_join": [_ctx, _i, _p, _i],
     "pb_capture_begin": [_ctx, _i],
     "pb_capture_end": [_ctx, _i, C.POINTER(C.c_void_p)],
     "pb_graph_launch": [_ctx, _i, C.c_void_p],

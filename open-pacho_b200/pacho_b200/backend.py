@@ -56,6 +56,25 @@ class DeviceBuffer:
             pass
 
 
+class BorrowedBuffer:
+    """Device memory that another library owns (``B200Backend.view``): used in
+    place, kept alive through ``owner`` and never freed here."""
+
+    __slots__ = ("backend", "ptr", "nbytes", "owner", "__weakref__")
+
+    def __init__(self, backend: "B200Backend", ptr: int, nbytes: int, owner):
+        self.backend = backend
+        self.ptr = ptr
+        self.nbytes = nbytes
+        self.owner = owner
+
+    def __int__(self):
+        return self.ptr
+
+    def release(self):
+        self.ptr, self.owner = 0, None
+
+
 class DeviceArray:
     """A typed view of one :class:`DeviceBuffer`: the four attributes the
     backend protocol reads of an operand (``shape``, ``ndim``, ``dtype``,
@@ -300,6 +319,67 @@ class B200Backend:
                 "pb_d2h",
             )
         return out
+
+    def view(self, obj, *, stream=None):
+        """A :class:`DeviceArray` over device memory that another library in
+        this process owns: any object with ``__cuda_array_interface__`` (a
+        PyTorch or CuPy array), C-contiguous, bool, float32 or float64, on
+        this backend's GPU and 16-byte aligned.  Nothing is copied, and the
+        array can be an operand or the ``out`` of a call.
+
+        This backend's stream first waits for the work queued so far on
+        ``stream`` (a ``cudaStream_t`` handle); by default on the stream that
+        the interface names, or on the legacy default stream where it names
+        none.  Later work of the owner is ordered with ``wait_stream`` and
+        ``signal_stream``.  Keep the owner from reusing the memory until the
+        calls on it have finished, or until its stream has been signalled."""
+        face = obj.__cuda_array_interface__
+        dtype = self.validate_dtype(face["typestr"])
+        shape = tuple(int(d) for d in face["shape"])
+        ptr, read_only = face["data"]
+        if read_only:
+            raise ValueError("b200 view needs writable memory")
+        strides = face.get("strides")
+        if strides is not None and prod(shape):
+            step = dtype.itemsize
+            for dim, stride in zip(reversed(shape), reversed(tuple(strides))):
+                if dim != 1 and stride != step:
+                    raise ValueError("b200 view needs C-contiguous memory")
+                step *= dim
+        nbytes = prod(shape) * dtype.itemsize
+        if nbytes and ptr % 16:
+            raise ValueError("b200 view needs 16-byte aligned memory")
+        with self._lock:
+            self._require_open()
+            if nbytes:
+                self._check(self._lib.pb_pointer_check(self._ctx, 0, C.c_void_p(ptr), nbytes),
+                            "pb_pointer_check")
+            if stream is None:
+                # Version 3 names the stream; None there asks for no ordering.
+                stream = face.get("stream", 0)
+                if stream is not None:
+                    self.wait_stream(stream)
+            else:
+                self.wait_stream(stream)
+        buf = BorrowedBuffer(self, int(ptr or 0), nbytes, obj)
+        self._buffers.add(buf)
+        return DeviceArray(self, buf, shape, dtype)
+
+    def wait_stream(self, stream=0):
+        """Order this backend's later work after the work queued so far on
+        ``stream`` (a ``cudaStream_t`` handle of this GPU; 0: the legacy default
+        stream).  The host does not wait."""
+        self._join(stream, _lib.PB_JOIN_WAIT)
+
+    def signal_stream(self, stream=0):
+        """Order ``stream``'s later work after this backend's work so far."""
+        self._join(stream, _lib.PB_JOIN_SIGNAL)
+
+    def _join(self, stream, direction):
+        with self._lock:
+            self._require_open()
+            self._check(self._lib.pb_stream_join(self._ctx, 0, C.c_void_p(int(stream) or None), direction),
+                        "pb_stream_join")
 
     def release_cached_memory(self):
         with self._lock:
