@@ -375,6 +375,81 @@ enum { PB_REDUCE_SUM = 0, PB_REDUCE_MIN = 1, PB_REDUCE_MAX = 2 };
 int pb_reduce(pb_ctx* ctx, int dev, int op, int in_dtype, const void* src, int ndim,
               const int64_t* shape, uint32_t axes_mask, int out_dtype, void* out);
 
+/* ---- along an axis, and over many tensors: layers and their training step -- *
+ * None of these has a counterpart in the reference, which has no operation
+ * that carries a value along an axis, no normalisation and no gradients.  Their
+ * outputs overlap neither each other nor an input, except where an entry
+ * says so (PB_ERR_INVALID). */
+
+/* Gated linear recurrence along the middle axis of the contiguous view
+ * (outer, length, inner), for every o < outer and i < inner:
+ *     h[o,t,i] = alpha[o,t,i] * h[o,t-1,i] + u[o,t,i],   h[o,-1,i] = state[o,i]
+ * PB_GATE_LINEAR: alpha = a, u = b.  PB_GATE_SIGMOID: `a` holds logits,
+ * alpha = 1 / (1 + exp(-a)) and u = (1 - alpha) * b.  `state` NULL is zero.
+ * `final` (outer, inner; NULL: not wanted) receives h[o,length-1,i], or the
+ * state when length == 0; final may be the same memory as state, which is
+ * how a stream of single steps keeps its state.  Long sequences of few
+ * columns are cut into chunks whose combined steps are carried in float64;
+ * the result does not depend on the order in which they run.  Gates are meant
+ * to be finite: behind a NaN or an Inf in a or b of its column, h is not finite
+ * as long as the recurrence written above would not be, but which of the two
+ * it is may differ. */
+enum { PB_GATE_LINEAR = 0, PB_GATE_SIGMOID = 1 };
+int pb_recurrence(pb_ctx* ctx, int dev, int dtype, int gate, int64_t outer, int64_t length,
+                  int64_t inner, const void* a, const void* b, const void* state, void* h,
+                  void* final);
+
+/* Gradients of pb_recurrence: with h its output, dh the gradient of h and
+ * dfinal (NULL: zero) that of `final`,
+ *     g[t] = dh[t] + alpha[t+1] * g[t+1],   g[length-1] = dh[length-1] + dfinal
+ * PB_GATE_LINEAR: db = g, da = g * h[t-1] (b is not read and may be NULL).
+ * PB_GATE_SIGMOID: db = g (1 - alpha), da = g (h[t-1] - b) alpha (1 - alpha).
+ * dstate (NULL: not wanted) = alpha[0] * g[0], or dfinal when length == 0.
+ * h[-1] is `state`, as given to pb_recurrence. */
+int pb_recurrence_backward(pb_ctx* ctx, int dev, int dtype, int gate, int64_t outer,
+                           int64_t length, int64_t inner, const void* a, const void* b,
+                           const void* h, const void* dh, const void* state,
+                           const void* dfinal, void* da, void* db, void* dstate);
+
+/* Group norm with an activation, channels last: x is (N, S, C) with C = G * m;
+ * for each n and group g, over its S * m values,
+ *     y = act((x - mean) * rstd * weight[c] + bias[c]),  rstd = 1 / sqrt(var + eps)
+ * with the variance of the whole set (divided by S * m).  weight and bias
+ * (C values; NULL: ones, zeros) are independent of each other.  mean and rstd
+ * (N * G values; NULL: not wanted) receive the statistics, which are summed
+ * in float64.  PB_ACT_GELU is z * Phi(z) with the normal distribution's Phi.
+ * G = 1 with S = 1 is a layer norm of rows of C.  S == 0 or C == 0 is an error. */
+enum { PB_ACT_NONE = 0, PB_ACT_RELU = 1, PB_ACT_SILU = 2, PB_ACT_GELU = 3 };
+int pb_group_norm(pb_ctx* ctx, int dev, int dtype, int act, int64_t N, int64_t S, int64_t C,
+                  int64_t G, double eps, const void* x, const void* weight, const void* bias,
+                  void* y, void* mean, void* rstd);
+
+/* Gradients of pb_group_norm at the same x, weight and bias, with the mean and
+ * rstd it returned.  dx is (N, S, C); dweight and dbias (C values; NULL: not
+ * wanted, N == 0: zeros) are sums over N and S, accumulated in float64 in a
+ * fixed order.  The derivative of PB_ACT_RELU at 0 is 0. */
+int pb_group_norm_backward(pb_ctx* ctx, int dev, int dtype, int act, int64_t N, int64_t S,
+                           int64_t C, int64_t G, const void* dy, const void* x,
+                           const void* mean, const void* rstd, const void* weight,
+                           const void* bias, void* dx, void* dweight, void* dbias);
+
+/* One AdamW step over `count` tensors at once (decoupled weight decay), in
+ * place; tensor j has sizes[j] values (0 allowed) in params[j], grads[j] and
+ * the two moments exp_avg[j], exp_avg_sq[j], all of `dtype`:
+ *     g = grad * (*grad_scale)        (device scalar of dtype; NULL: 1)
+ *     m = beta1 m + (1 - beta1) g;    v = beta2 v + (1 - beta2) g^2
+ *     p = p (1 - lr weight_decay) - lr / (1 - beta1^step) *
+ *         m / (sqrt(v / (1 - beta2^step)) + eps)
+ * `step` counts from 1.  A few launches do all tensors (one per 512).  The
+ * four pointer arrays and sizes are host memory, read before the call returns.
+ * No params, exp_avg or exp_avg_sq may overlap another or a gradient.  lr and
+ * step are values of the call, so a captured call would repeat them:
+ * PB_ERR_UNSUPPORTED during a capture. */
+int pb_adamw(pb_ctx* ctx, int dev, int dtype, int64_t count, void* const* params,
+             const void* const* grads, void* const* exp_avg, void* const* exp_avg_sq,
+             const int64_t* sizes, double lr, double beta1, double beta2, double eps,
+             double weight_decay, int64_t step, const void* grad_scale);
+
 /* ---- multi-GPU (one process per GPU; NCCL loaded on first use) --------- *
  * None of these has a counterpart in the reference, which is single-device
  * (src/openpacho/_cuda.py:138-199). */

@@ -1,0 +1,402 @@
+// Group norm with an activation, channels last, and its gradients (HBM-bound:
+// forward 2 values moved per element, backward 3).
+//
+// x is (N, S, C), C = G groups of m channels; a group's set is its m channels
+// over the S positions of one sample.  Channels are contiguous, so lanes run
+// over channels and every sum over positions is a sum down a column:
+//   sums   each block takes a run of positions of one sample and adds up two
+//          numbers per channel in float64 (forward: x - k and (x - k)^2 with
+//          the shift k = the group's first value, which keeps the variance of
+//          values far from zero; backward: dz and dz * xhat).  The block that
+//          finishes a sample last adds the blocks' sums in block order and then
+//          the channels of each group, so the result is deterministic.
+//   apply  a second pass over the same positions.
+// The statistics pass is what the algorithm cannot avoid reading twice for: the
+// second read comes from L2 while a sample is still there.
+#include "pb_layers.cuh"
+
+namespace pb {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T>
+struct NormArgs {
+  const T *x, *dy, *weight, *bias;
+  T* out;             // y or dx
+  T *mean, *rstd;     // forward: outputs, may be null; backward: inputs
+  T *dweight, *dbias; // may be null
+  double2* part;      // (N, chunks, C): per-channel sums of a block
+  double2* chan;      // (N, C): per-channel sums of a sample
+  double2* group;     // (N, G): forward (mean, rstd); backward (mean of w dz, mean of w dz xhat)
+  unsigned* arrivals; // N words, zero on entry and exit
+  int64_t N, S, C, G, m;
+  int64_t rows;       // positions per block
+  int64_t chunks;     // blocks per sample
+  double eps;
+};
+
+template <typename T, int ACT>
+__device__ __forceinline__ T activate(T z) {
+  if constexpr (ACT == PB_ACT_RELU) return z < T(0) ? T(0) : z;
+  if constexpr (ACT == PB_ACT_SILU) {
+    T s, rest;
+    sigmoid_pair(z, &s, &rest);
+    return z * s;
+  }
+  if constexpr (ACT == PB_ACT_GELU) {
+    // z Phi(z) with Phi(z) = erfc(-z / sqrt 2) / 2, which keeps its relative
+    // accuracy for negative z where 1 + erf would cancel.
+    if constexpr (sizeof(T) == 4) return z * (0.5f * erfcf(z * -0.70710678118654752f));
+    else return z * (0.5 * erfc(z * -0.70710678118654752));
+  }
+  return z;
+}
+
+template <typename T, int ACT>
+__device__ __forceinline__ T slope(T z) {
+  if constexpr (ACT == PB_ACT_RELU) return z > T(0) ? T(1) : T(0);
+  if constexpr (ACT == PB_ACT_SILU) {
+    T s, rest;
+    sigmoid_pair(z, &s, &rest);
+    return s * fma(z, rest, T(1));
+  }
+  if constexpr (ACT == PB_ACT_GELU) {
+    const T phi = exp_of(T(-0.5) * z * z) * T(0.39894228040143268);
+    if constexpr (sizeof(T) == 4) return fmaf(z, phi, 0.5f * erfcf(z * -0.70710678118654752f));
+    else return fma(z, phi, 0.5 * erfc(z * -0.70710678118654752));
+  }
+  return T(1);
+}
+
+// The shift of a group's sums: its first value, or 0 where that is not finite
+// (a non-finite shift would hide which of NaN and Inf the mean is).
+template <typename T>
+__device__ __forceinline__ double shift_of(const NormArgs<T>& p, int64_t n, int64_t g) {
+  const double k = (double)__ldg(p.x + n * p.S * p.C + g * p.m);
+  return isfinite(k) ? k : 0.0;
+}
+
+// Sums pass.  Threads form tx lanes over packs of V channels and ty rows.
+template <typename T, int V, int ACT, bool BWD>
+__global__ void __launch_bounds__(kThreads) norm_sums_kernel(const NormArgs<T> p, int tx, int ty) {
+  __shared__ double2 red[kThreads];
+  __shared__ bool last;
+  const int lx = threadIdx.x % tx, ly = threadIdx.x / tx;
+  for (int64_t unit = blockIdx.x; unit < p.N * p.chunks; unit += gridDim.x) {
+    const int64_t n = unit / p.chunks, chunk = unit % p.chunks;
+    const int64_t r0 = chunk * p.rows, r1 = min(p.S, r0 + p.rows);
+    double2* const part = p.part + unit * p.C;
+    for (int64_t c0 = 0; c0 < p.C; c0 += (int64_t)tx * V) {
+      const int64_t c = c0 + (int64_t)lx * V;
+      const bool on = ly < ty && c < p.C;
+      double s1[V] = {}, s2[V] = {};
+      if (on) {
+        double k[V];
+        T mean[V], rstd[V], w[V], b[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int64_t g = (c + i) / p.m;
+          if constexpr (BWD) {
+            mean[i] = __ldg(p.mean + n * p.G + g);
+            rstd[i] = __ldg(p.rstd + n * p.G + g);
+            w[i] = p.weight ? __ldg(p.weight + c + i) : T(1);
+            b[i] = p.bias ? __ldg(p.bias + c + i) : T(0);
+          } else {
+            k[i] = shift_of(p, n, g);
+          }
+        }
+        const T* x = p.x + (n * p.S + r0 + ly) * p.C + c;
+        const T* dy = BWD ? p.dy + (n * p.S + r0 + ly) * p.C + c : nullptr;
+#pragma unroll 4
+        for (int64_t r = r0 + ly; r < r1; r += ty) {
+          const Pack<T, V> q = load_pack<T, V>(x);
+          x += ty * p.C;
+          if constexpr (BWD) {
+            const Pack<T, V> e = load_pack<T, V>(dy);
+            dy += ty * p.C;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const T xh = (q.v[i] - mean[i]) * rstd[i];
+              const T dz = e.v[i] * slope<T, ACT>(fma(xh, w[i], b[i]));
+              s1[i] += (double)dz;
+              s2[i] += (double)(dz * xh);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const double v = (double)q.v[i] - k[i];
+              s1[i] += v;
+              s2[i] = fma(v, v, s2[i]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        __syncthreads();
+        red[threadIdx.x] = make_double2(s1[i], s2[i]);
+        __syncthreads();
+        if (on && ly == 0) {
+          double2 t = red[lx];
+          for (int y = 1; y < ty; ++y) {
+            t.x += red[y * tx + lx].x;
+            t.y += red[y * tx + lx].y;
+          }
+          part[c + i] = t;
+        }
+      }
+    }
+    // The last block of the sample adds up the blocks' sums.
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = p.chunks == 1 || atomicAdd(&p.arrivals[n], 1u) == (unsigned)p.chunks - 1;
+    __syncthreads();
+    if (!last) continue;
+    __threadfence();
+    for (int64_t c = threadIdx.x; c < p.C; c += kThreads) {
+      double2 t = make_double2(0.0, 0.0);
+      const double2* q = p.part + n * p.chunks * p.C + c;
+      for (int64_t k = 0; k < p.chunks; ++k, q += p.C) {
+        const double2 v = __ldcg(q);
+        t.x += v.x;
+        t.y += v.y;
+      }
+      p.chan[n * p.C + c] = t;
+    }
+    __syncthreads();
+    const double count = (double)p.S * (double)p.m;
+    for (int64_t g = threadIdx.x; g < p.G; g += kThreads) {
+      double2 t = make_double2(0.0, 0.0);
+      for (int64_t c = g * p.m; c < (g + 1) * p.m; ++c) {
+        const double2 v = p.chan[n * p.C + c];
+        const double w = BWD && p.weight ? (double)__ldg(p.weight + c) : 1.0;
+        t.x = fma(w, v.x, t.x);
+        t.y = fma(w, v.y, t.y);
+      }
+      t.x /= count;
+      t.y /= count;
+      if constexpr (!BWD) {
+        // A set with NaN or Inf in it has a NaN variance (fmax alone would drop
+        // it); finite float64 values whose squares overflow have an infinite one.
+        const double var = isinf(t.y) ? t.y : fmax(fma(-t.x, t.x, t.y), 0.0);
+        const double rstd = isfinite(t.x) ? 1.0 / sqrt(var + p.eps) : t.x - t.x;
+        t = make_double2(t.x + shift_of(p, n, g), rstd);
+        if (p.mean) p.mean[n * p.G + g] = (T)t.x;
+        if (p.rstd) p.rstd[n * p.G + g] = (T)t.y;
+      }
+      p.group[n * p.G + g] = t;
+    }
+    if (threadIdx.x == 0 && p.chunks > 1) p.arrivals[n] = 0;
+    __syncthreads();
+  }
+}
+
+template <typename T, int V, int ACT, bool BWD>
+__global__ void __launch_bounds__(kThreads) norm_apply_kernel(const NormArgs<T> p, int tx, int ty) {
+  const int lx = threadIdx.x % tx, ly = threadIdx.x / tx;
+  for (int64_t unit = blockIdx.x; unit < p.N * p.chunks; unit += gridDim.x) {
+    const int64_t n = unit / p.chunks, chunk = unit % p.chunks;
+    const int64_t r0 = chunk * p.rows, r1 = min(p.S, r0 + p.rows);
+    for (int64_t c = (int64_t)lx * V; c < p.C && ly < ty; c += (int64_t)tx * V) {
+      T mean[V], low[V], rstd[V], w[V], b[V], m1[V], m2[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int64_t g = (c + i) / p.m;
+        const double2 t = p.group[n * p.G + g];
+        w[i] = p.weight ? __ldg(p.weight + c + i) : T(1);
+        b[i] = p.bias ? __ldg(p.bias + c + i) : T(0);
+        if constexpr (BWD) {
+          mean[i] = __ldg(p.mean + n * p.G + g);
+          rstd[i] = __ldg(p.rstd + n * p.G + g);
+          m1[i] = (T)t.x;
+          m2[i] = (T)t.y;
+        } else {
+          // The mean in two parts, so that its rounding does not show where
+          // the values lie far from zero.
+          mean[i] = (T)t.x;
+          low[i] = (T)(t.x - (double)mean[i]);
+          rstd[i] = (T)t.y;
+        }
+      }
+      int64_t at = (n * p.S + r0 + ly) * p.C + c;
+#pragma unroll 4
+      for (int64_t r = r0 + ly; r < r1; r += ty, at += ty * p.C) {
+        const Pack<T, V> q = load_pack<T, V>(p.x + at);
+        Pack<T, V> o;
+        if constexpr (BWD) {
+          const Pack<T, V> e = load_pack<T, V>(p.dy + at);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const T xh = (q.v[i] - mean[i]) * rstd[i];
+            const T dz = e.v[i] * slope<T, ACT>(fma(xh, w[i], b[i]));
+            o.v[i] = rstd[i] * (fma(w[i], dz, -m1[i]) - xh * m2[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const T xh = ((q.v[i] - mean[i]) - low[i]) * rstd[i];
+            o.v[i] = activate<T, ACT>(fma(xh, w[i], b[i]));
+          }
+        }
+        store_pack<T, V>(p.out + at, o);
+      }
+    }
+  }
+}
+
+// dweight and dbias: the samples' per-channel sums in sample order.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) norm_affine_kernel(const NormArgs<T> p) {
+  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (c >= p.C) return;
+  double2 t = make_double2(0.0, 0.0);
+  for (int64_t n = 0; n < p.N; ++n) {
+    const double2 v = p.chan[n * p.C + c];
+    t.x += v.x;
+    t.y += v.y;
+  }
+  if (p.dbias) p.dbias[c] = (T)t.x;
+  if (p.dweight) p.dweight[c] = (T)t.y;
+}
+
+template <typename T, int V, int ACT, bool BWD>
+int launch(Device* d, NormArgs<T> p) {
+  const int64_t lanes = ceil_div(p.C, (int64_t)V);
+  const int tx = (int)(lanes < kThreads ? lanes : kThreads), ty = kThreads / tx;
+  // Blocks of at least 16 positions per thread, about eight per SM in all.
+  int64_t chunks = ceil_div((int64_t)d->sm_count * 8, p.N);
+  const int64_t most = ceil_div(p.S, (int64_t)ty * 16);
+  if (chunks > most) chunks = most;
+  p.rows = ceil_div(p.S, chunks);
+  p.chunks = ceil_div(p.S, p.rows);
+  size_t part, chan, group;
+  const int64_t e1[] = {p.N, p.chunks, p.C}, e2[] = {p.N, p.C}, e3[] = {p.N, p.G};
+  if (!array_bytes(e1, 3, sizeof(double2), &part) || !array_bytes(e2, 2, sizeof(double2), &chan) ||
+      !array_bytes(e3, 2, sizeof(double2), &group))
+    PB_FAIL(PB_ERR_INVALID, "extents too large");
+  void* ws;
+  PB_CHECK(scratch(d, part + chan + group, &ws));
+  p.part = static_cast<double2*>(ws);
+  p.chan = p.part + part / sizeof(double2);
+  p.group = p.chan + chan / sizeof(double2);
+  if (p.chunks > 1) PB_CHECK(counters(d, (size_t)p.N, &p.arrivals));
+  const int64_t units = p.N * p.chunks, cap = int64_t(1) << 30;
+  const unsigned grid = (unsigned)(units < cap ? units : cap);
+  PB_CHECK(kt_begin(d));
+  norm_sums_kernel<T, V, ACT, BWD><<<grid, kThreads, 0, d->stream>>>(p, tx, ty);
+  PB_LAUNCHED(d);
+  norm_apply_kernel<T, V, ACT, BWD><<<grid, kThreads, 0, d->stream>>>(p, tx, ty);
+  PB_LAUNCHED(d);
+  PB_CHECK(kt_end(d));
+  if (BWD && (p.dweight || p.dbias)) {
+    norm_affine_kernel<T><<<(unsigned)ceil_div(p.C, (int64_t)kThreads), kThreads, 0, d->stream>>>(p);
+    PB_LAUNCHED(d);
+  }
+  return PB_OK;
+}
+
+template <typename T, int V, bool BWD>
+int launch_act(Device* d, int act, const NormArgs<T>& p) {
+  switch (act) {
+    case PB_ACT_RELU: return launch<T, V, PB_ACT_RELU, BWD>(d, p);
+    case PB_ACT_SILU: return launch<T, V, PB_ACT_SILU, BWD>(d, p);
+    case PB_ACT_GELU: return launch<T, V, PB_ACT_GELU, BWD>(d, p);
+    default: return launch<T, V, PB_ACT_NONE, BWD>(d, p);
+  }
+}
+
+struct Pointers {
+  const void *x, *dy, *weight, *bias;
+  void *out, *mean, *rstd, *dweight, *dbias;
+};
+
+template <typename T, bool BWD>
+int dispatch(Device* d, int act, int64_t N, int64_t S, int64_t C, int64_t G, double eps, const Pointers& q) {
+  NormArgs<T> p = {};
+  p.x = static_cast<const T*>(q.x);
+  p.dy = static_cast<const T*>(q.dy);
+  p.weight = static_cast<const T*>(q.weight);
+  p.bias = static_cast<const T*>(q.bias);
+  p.out = static_cast<T*>(q.out);
+  p.mean = static_cast<T*>(q.mean);
+  p.rstd = static_cast<T*>(q.rstd);
+  p.dweight = static_cast<T*>(q.dweight);
+  p.dbias = static_cast<T*>(q.dbias);
+  p.N = N;
+  p.S = S;
+  p.C = C;
+  p.G = G;
+  p.m = C / G;
+  p.eps = eps;
+  constexpr int V = Vec16<T>::n;
+  const bool wide = C % V == 0 && (((uintptr_t)q.x | (uintptr_t)q.dy | (uintptr_t)q.out) & 15) == 0;
+  return wide ? launch_act<T, V, BWD>(d, act, p) : launch_act<T, 1, BWD>(d, act, p);
+}
+
+// Checks common to both directions; the bytes of x and of one sample's statistics.
+int check_view(pb_ctx* ctx, int dtype, int act, int64_t N, int64_t S, int64_t C, int64_t G, size_t* bytes,
+               size_t* stats) {
+  if (!ctx) PB_FAIL(PB_ERR_INVALID, "null context");
+  if (dtype != PB_F32 && dtype != PB_F64) PB_FAIL(PB_ERR_INVALID, "group norm takes float32 or float64");
+  if (act < PB_ACT_NONE || act > PB_ACT_GELU) PB_FAIL(PB_ERR_INVALID, "unknown activation %d", act);
+  if (N < 0 || S < 0 || C < 0) PB_FAIL(PB_ERR_INVALID, "negative extent");
+  if (G < 1 || C % G) PB_FAIL(PB_ERR_INVALID, "%lld channels do not divide into %lld groups", (long long)C, (long long)G);
+  if (!S || !C) PB_FAIL(PB_ERR_INVALID, "group norm of an empty set");
+  const size_t item = dtype == PB_F32 ? 4 : 8;
+  const int64_t all[3] = {N, S, C}, ends[2] = {N, G};
+  if (!array_bytes(all, 3, item, bytes) || !array_bytes(ends, 2, item, stats))
+    PB_FAIL(PB_ERR_INVALID, "extents too large");
+  return PB_OK;
+}
+
+}  // namespace
+}  // namespace pb
+
+using namespace pb;
+
+extern "C" {
+
+int pb_group_norm(pb_ctx* ctx, int dev, int dtype, int act, int64_t N, int64_t S, int64_t C, int64_t G, double eps,
+                  const void* x, const void* weight, const void* bias, void* y, void* mean, void* rstd) {
+  size_t bytes, stats;
+  PB_CHECK(check_view(ctx, dtype, act, N, S, C, G, &bytes, &stats));
+  if (!(eps >= 0.0)) PB_FAIL(PB_ERR_INVALID, "eps is not negative");
+  if (!N) return PB_OK;
+  if (!x || !y) PB_FAIL(PB_ERR_INVALID, "null operand");
+  const size_t item = dtype == PB_F32 ? 4 : 8, line = (size_t)C * item;
+  const Span in[] = {{x, bytes}, {weight, line}, {bias, line}};
+  const Span out[] = {{y, bytes}, {mean, stats}, {rstd, stats}};
+  PB_CHECK(check_operands(out, 3, in, 3, item));
+  std::lock_guard<std::recursive_mutex> g(ctx->mu);
+  Device* d;
+  PB_CHECK(enter(ctx, dev, &d));
+  const Pointers q = {x, nullptr, weight, bias, y, mean, rstd, nullptr, nullptr};
+  return dtype == PB_F32 ? dispatch<float, false>(d, act, N, S, C, G, eps, q)
+                         : dispatch<double, false>(d, act, N, S, C, G, eps, q);
+}
+
+int pb_group_norm_backward(pb_ctx* ctx, int dev, int dtype, int act, int64_t N, int64_t S, int64_t C, int64_t G,
+                           const void* dy, const void* x, const void* mean, const void* rstd, const void* weight,
+                           const void* bias, void* dx, void* dweight, void* dbias) {
+  size_t bytes, stats;
+  PB_CHECK(check_view(ctx, dtype, act, N, S, C, G, &bytes, &stats));
+  const size_t item = dtype == PB_F32 ? 4 : 8, line = (size_t)C * item;
+  if (N && (!dy || !x || !mean || !rstd || !dx)) PB_FAIL(PB_ERR_INVALID, "null operand");
+  const Span in[] = {{dy, bytes}, {x, bytes}, {mean, stats}, {rstd, stats}, {weight, line}, {bias, line}};
+  const Span out[] = {{dx, bytes}, {dweight, line}, {dbias, line}};
+  PB_CHECK(check_operands(out, 3, in, 6, item));
+  std::lock_guard<std::recursive_mutex> g(ctx->mu);
+  Device* d;
+  PB_CHECK(enter(ctx, dev, &d));
+  if (!N) {
+    for (void* q : {dweight, dbias})
+      if (q) PB_CHECK(fill_device(d, dtype, q, (size_t)C, 0.0));
+    return PB_OK;
+  }
+  const Pointers q = {x, dy, weight, bias, dx, const_cast<void*>(mean), const_cast<void*>(rstd), dweight, dbias};
+  return dtype == PB_F32 ? dispatch<float, true>(d, act, N, S, C, G, 0.0, q)
+                         : dispatch<double, true>(d, act, N, S, C, G, 0.0, q);
+}
+
+}  // extern "C"

@@ -1,0 +1,98 @@
+// Helpers shared by the layer kernels (recurrence, group norm, AdamW).
+#pragma once
+
+#include "pb_internal.cuh"
+
+namespace pb {
+
+template <typename T> struct Vec16;
+template <> struct Vec16<float> { using type = float4; static constexpr int n = 4; };
+template <> struct Vec16<double> { using type = double2; static constexpr int n = 2; };
+
+// V values of T in registers, moved with one access when V * sizeof(T) is 16
+// (the address then has to be 16-byte aligned) and value by value otherwise.
+template <typename T, int V>
+struct Pack {
+  T v[V];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* __restrict__ p) {
+  Pack<T, V> r;
+  if constexpr (V * sizeof(T) == 16) {
+    const typename Vec16<T>::type q = __ldg(reinterpret_cast<const typename Vec16<T>::type*>(p));
+    __builtin_memcpy(&r, &q, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = __ldg(p + i);
+  }
+  return r;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& r) {
+  if constexpr (V * sizeof(T) == 16) {
+    typename Vec16<T>::type q;
+    __builtin_memcpy(&q, &r, 16);
+    *reinterpret_cast<typename Vec16<T>::type*>(p) = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) p[i] = r.v[i];
+  }
+}
+
+__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+__device__ __forceinline__ float reciprocal(float x) { return __fdividef(1.0f, x); }
+__device__ __forceinline__ double reciprocal(double x) { return 1.0 / x; }
+
+// s = 1 / (1 + e^-z) and rest = 1 - s, each to a few roundings of its own size:
+// with e = e^-|z| <= 1 the two are 1/(1+e) and e/(1+e), so neither is the
+// difference of two nearly equal numbers.  1 + e lies in [1, 2], where the
+// fast float32 division is within 2 ulp.
+template <typename T>
+__device__ __forceinline__ void sigmoid_pair(T z, T* s, T* rest) {
+  const T e = exp_of(z < T(0) ? z : -z);
+  const T big = reciprocal(T(1) + e), small = e * big;
+  const bool neg = z < T(0);
+  *s = neg ? small : big;
+  *rest = neg ? big : small;
+}
+
+// Whether [p, p + pn) and [q, q + qn) share a byte (NULL shares none).
+inline bool overlap(const void* p, size_t pn, const void* q, size_t qn) {
+  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+  return p && q && pn && qn && a < b + qn && b < a + pn;
+}
+
+struct Span {
+  const void* p;
+  size_t n;
+};
+// Refuses an output that overlaps another output or an input, and an operand
+// that does not start on a whole element.
+inline int check_operands(const Span* out, int nout, const Span* in, int nin, size_t item) {
+  for (int i = 0; i < nout; ++i) {
+    for (int j = i + 1; j < nout; ++j)
+      if (overlap(out[i].p, out[i].n, out[j].p, out[j].n)) PB_FAIL(PB_ERR_INVALID, "two outputs overlap");
+    for (int j = 0; j < nin; ++j)
+      if (overlap(out[i].p, out[i].n, in[j].p, in[j].n)) PB_FAIL(PB_ERR_INVALID, "an output overlaps an input");
+    if ((uintptr_t)out[i].p % item) PB_FAIL(PB_ERR_INVALID, "a pointer is not aligned to its type");
+  }
+  for (int j = 0; j < nin; ++j)
+    if ((uintptr_t)in[j].p % item) PB_FAIL(PB_ERR_INVALID, "a pointer is not aligned to its type");
+  return PB_OK;
+}
+
+// Product of extents of one array in bytes; false when it passes 2^62.
+inline bool array_bytes(const int64_t* extents, int n, size_t item, size_t* bytes) {
+  unsigned __int128 t = item;
+  for (int i = 0; i < n; ++i) {
+    t *= (uint64_t)extents[i];
+    if (t > ((unsigned __int128)1 << 62)) return false;
+  }
+  *bytes = (size_t)t;
+  return true;
+}
+
+}  // namespace pb

@@ -11,6 +11,8 @@
   command (``python -m pacho_b200``) run on the B200.
 * :mod:`pacho_b200.distributed` -- the sharded forms (batch split, row blocks
   with B broadcast, norm and DOT partials over NVLink) for one process per GPU.
+* :mod:`pacho_b200.layers` -- :func:`linear_recurrence`, :func:`group_norm`, their
+  backward passes and :class:`AdamW`: a sequence layer and its training step.
 * :func:`devices` -- the visible B200s as OpenPacho-style ``DeviceInfo``.
 * :class:`DeviceArray` -- a typed view of a device buffer, returned by this
   package's own functions when they are not handed OpenPacho arrays.
@@ -19,11 +21,19 @@
 from .backend import B200Backend, DeviceArray, DeviceBuffer
 from .discovery import DeviceInfo, devices
 from .exceptions import BackendMismatchError, BackendUnavailableError, UnsupportedDtypeError
+from .layers import (
+    AdamW,
+    group_norm,
+    group_norm_backward,
+    linear_recurrence,
+    linear_recurrence_backward,
+)
 from .register import register, unregister
 
 __version__ = "0.2.0"
 
 __all__ = [
+    "AdamW",
     "B200Backend",
     "BackendMismatchError",
     "BackendUnavailableError",
@@ -32,6 +42,10 @@ __all__ = [
     "DeviceInfo",
     "UnsupportedDtypeError",
     "devices",
+    "group_norm",
+    "group_norm_backward",
+    "linear_recurrence",
+    "linear_recurrence_backward",
     "register",
     "unregister",
 ]

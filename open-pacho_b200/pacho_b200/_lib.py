@@ -36,6 +36,11 @@ PB_GEMM_TF32X3_PRESPLIT = 4
 PB_GEMM_TF32X3_FUSED = 5
 PB_GEMM_SKINNY = 6
 
+# Gates of the linear recurrence and activations of the group norm (PB_GATE_*,
+# PB_ACT_*).
+GATES = {"linear": 0, "sigmoid": 1}
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
+
 PB_JOIN_WAIT = 0
 PB_JOIN_SIGNAL = 1
 
@@ -106,6 +111,12 @@ PROTOTYPES = {
     "pb_elementwise": [_ctx, _i, _i, _i, C.POINTER(_p), C.POINTER(_i), _pi64, _i, _pi64, _i, _p],
     "pb_gather": [_ctx, _i, _i, _p, _i, _pi64, _i64, _pi64, _p],
     "pb_reduce": [_ctx, _i, _i, _i, _p, _i, _pi64, C.c_uint32, _i, _p],
+    "pb_recurrence": [_ctx, _i, _i, _i, _i64, _i64, _i64, _p, _p, _p, _p, _p],
+    "pb_recurrence_backward": [_ctx, _i, _i, _i, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p],
+    "pb_group_norm": [_ctx, _i, _i, _i, _i64, _i64, _i64, _i64, C.c_double, _p, _p, _p, _p, _p, _p],
+    "pb_group_norm_backward": [_ctx, _i, _i, _i, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p],
+    "pb_adamw": [_ctx, _i, _i, _i64, C.POINTER(_p), C.POINTER(_p), C.POINTER(_p), C.POINTER(_p), _pi64,
+                 C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _i64, _p],
     "pb_dot": [_ctx, _i, _i, _i64, _p, _p, _p],
     "pb_dot_noalloc": [_ctx, _i, _i, _i64, _p, _p, _p],
     "pb_peer_export": [_ctx, _i, _i, _i, C.c_char_p],
