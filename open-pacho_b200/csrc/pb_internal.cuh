@@ -87,6 +87,11 @@ struct Device {
   unsigned int* tags = nullptr;
   size_t tags_n = 0;
   unsigned int tag_gen = 0;
+  // Ticket, epoch and flags of the cut recurrence, zeroed when allocated: a flag
+  // is set when it holds the launch's epoch, which the launch itself advances
+  // at its end, so nothing clears it and a replayed graph gets a new one.
+  unsigned int* epochs = nullptr;
+  size_t epochs_n = 0;
   // Kernel error word in mapped, pinned host memory (no copy needed to read it).
   int* err_host = nullptr;
   int* err_dev = nullptr;
@@ -145,6 +150,8 @@ int check_kernel_error(Device* d);
 int scratch(Device* d, size_t bytes, void** out);
 // Ensure at least `n` zeroed counters; returns the pointer.
 int counters(Device* d, size_t n, unsigned int** out);
+// Ensure at least `n` words for a launch with epochs (see Device::epochs).
+int epoch_words(Device* d, size_t n, unsigned int** out);
 // Raise `kernel`'s dynamic shared-memory limit to `bytes` on d's device, once
 // per (kernel, device): the attribute is per device, so a context over
 // several devices sets it on each.  The device must be current (enter()).

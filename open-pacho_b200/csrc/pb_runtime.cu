@@ -103,6 +103,21 @@ int operand_tags(Device* d, size_t n, unsigned int** out, unsigned int* gen) {
   return PB_OK;
 }
 
+int epoch_words(Device* d, size_t n, unsigned int** out) {
+  if (n > d->epochs_n) {
+    PB_NO_GROWTH_IN_CAPTURE(d);
+    PB_CHECK(release_buffer(d, d->epochs));
+    d->epochs = nullptr;
+    d->epochs_n = 0;
+    const size_t want = n < 16384 ? 16384 : n;
+    PB_CUDA(cudaMallocAsync((void**)&d->epochs, want * sizeof(unsigned int), d->pool, d->stream));
+    PB_CUDA(cudaMemsetAsync(d->epochs, 0, want * sizeof(unsigned int), d->stream));
+    d->epochs_n = want;
+  }
+  *out = d->epochs;
+  return PB_OK;
+}
+
 constexpr size_t kMaxTimedLaunches = 4096;
 
 int kt_begin(Device* d) {
@@ -157,6 +172,9 @@ static void release_device(Device* d) {
   if (d->scratch) cudaFreeAsync(d->scratch, d->stream);
   if (d->counters) cudaFreeAsync(d->counters, d->stream);
   if (d->tags) cudaFreeAsync(d->tags, d->stream);
+  if (d->epochs) cudaFreeAsync(d->epochs, d->stream);
+  d->epochs = nullptr;
+  d->epochs_n = 0;
   for (void* p : d->retired) cudaFreeAsync(p, d->stream);
   d->retired.clear();
   if (d->stream) cudaStreamSynchronize(d->stream);
@@ -445,6 +463,9 @@ int pb_trim(pb_ctx* ctx, int dev) {
   if (d->tags) PB_CUDA(cudaFreeAsync(d->tags, d->stream));
   d->tags = nullptr;
   d->tags_n = 0;
+  if (d->epochs) PB_CUDA(cudaFreeAsync(d->epochs, d->stream));
+  d->epochs = nullptr;
+  d->epochs_n = 0;
   PB_CUDA(cudaStreamSynchronize(d->stream));
   PB_CUDA(cudaMemPoolTrimTo(d->pool, 0));
   return PB_OK;
