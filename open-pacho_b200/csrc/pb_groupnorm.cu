@@ -11,14 +11,20 @@
 //          finishes a sample last adds the blocks' sums in block order and then
 //          the channels of each group, so the result is deterministic.
 //   apply  a second pass over the same positions.
-// The statistics pass is what the algorithm cannot avoid reading twice for: the
-// second read comes from L2 while a sample is still there.
+// The second read comes from L2 while a sample is still there.
+//
+// With one position (S = 1: a norm of each token) a group is a row of m
+// contiguous values, which fits into the registers of a part of a warp, a warp
+// or a block: one pass reads it, forms its sums and writes the result.  Such a
+// part of the block stays with one group and walks over the samples, so that
+// weight and bias stay in registers and the sums of dweight and dbias are its own.
 #include "pb_layers.cuh"
 
 namespace pb {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
 
 template <typename T>
 struct NormArgs {
@@ -245,19 +251,270 @@ __global__ void __launch_bounds__(kThreads) norm_apply_kernel(const NormArgs<T> 
   }
 }
 
-// dweight and dbias: the samples' per-channel sums in sample order.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_affine_kernel(const NormArgs<T> p) {
-  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= p.C) return;
-  double2 t = make_double2(0.0, 0.0);
-  for (int64_t n = 0; n < p.N; ++n) {
-    const double2 v = p.chan[n * p.C + c];
-    t.x += v.x;
-    t.y += v.y;
+__device__ __forceinline__ T activate(int act, T z) {
+  switch (act) {
+    case PB_ACT_RELU: return activate<T, PB_ACT_RELU>(z);
+    case PB_ACT_SILU: return activate<T, PB_ACT_SILU>(z);
+    case PB_ACT_GELU: return activate<T, PB_ACT_GELU>(z);
+    default: return z;
   }
-  if (p.dbias) p.dbias[c] = (T)t.x;
-  if (p.dweight) p.dweight[c] = (T)t.y;
+}
+template <typename T>
+__device__ __forceinline__ T slope(int act, T z) {
+  switch (act) {
+    case PB_ACT_RELU: return slope<T, PB_ACT_RELU>(z);
+    case PB_ACT_SILU: return slope<T, PB_ACT_SILU>(z);
+    case PB_ACT_GELU: return slope<T, PB_ACT_GELU>(z);
+    default: return T(1);
+  }
+}
+
+// Sums of two numbers over the LANES threads that share a row, the same in
+// each of them and in a fixed order.
+template <int LANES>
+__device__ __forceinline__ double2 row_sum(double2 t) {
+#pragma unroll
+  for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) {
+    t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
+    t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
+  }
+  if constexpr (LANES > 32) {
+    __shared__ double2 part[kWarps];
+    __syncthreads();  // the last use of `part` is over
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = t;
+    __syncthreads();
+    t = part[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) {
+      t.x += part[w].x;
+      t.y += part[w].y;
+    }
+  }
+  return t;
+}
+
+// Rows of m values (S = 1): LANES threads hold a row, ITEMS packs of V values
+// each.  Threads are numbered in units of a warp, or of the block where a row
+// takes it; a unit works on group u % G of samples chunk * rows ...
+template <typename T, int V, int LANES, int ITEMS, bool BWD>
+__global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormArgs<T> p, int act) {
+  constexpr int UNIT = LANES < 32 ? 32 : LANES, SUBS = UNIT / LANES;
+  const int64_t unit = (int64_t)blockIdx.x * (kThreads / UNIT) + threadIdx.x / UNIT;
+  if (unit >= p.G * p.chunks) return;  // whole units only
+  const int64_t g = unit % p.G, chunk = unit / p.G;
+  const int lane = threadIdx.x % LANES, sub = threadIdx.x % UNIT / LANES;
+  const int64_t n0 = chunk * p.rows, n1 = min(p.N, n0 + p.rows);
+  T w[ITEMS][V], b[ITEMS][V];
+  bool on[ITEMS];
+  double dw[BWD ? ITEMS : 1][V], db[BWD ? ITEMS : 1][V];
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int64_t c = (int64_t)(k * LANES + lane) * V;
+    on[k] = c < p.m;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      w[k][i] = on[k] && p.weight ? __ldg(p.weight + g * p.m + c + i) : T(1);
+      b[k][i] = on[k] && p.bias ? __ldg(p.bias + g * p.m + c + i) : T(0);
+      if constexpr (BWD) dw[k][i] = db[k][i] = 0.0;
+    }
+  }
+  auto fetch = [&](const T* from, int64_t n, Pack<T, V>* to) {
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      to[k] = Pack<T, V>{};
+      if (on[k] && n < n1) to[k] = load_pack<T, V>(from + n * p.C + g * p.m + (k * LANES + lane) * V);
+    }
+  };
+  const double count = (double)p.m;
+  Pack<T, V> x[ITEMS], e[BWD ? ITEMS : 1], x1[ITEMS], e1[BWD ? ITEMS : 1];
+  T mean1 = T(0), rstd1 = T(0);
+  auto fetch_next = [&](int64_t n) {
+    fetch(p.x, n, x1);
+    if constexpr (BWD) {
+      fetch(p.dy, n, e1);
+      if (n < n1) {
+        mean1 = __ldg(p.mean + n * p.G + g);
+        rstd1 = __ldg(p.rstd + n * p.G + g);
+      }
+    }
+  };
+  fetch_next(n0 + sub);
+  // Every part of a unit makes the same number of turns: row_sum is theirs together.
+  for (int64_t n = n0 + sub, turns = (n1 - n0 + SUBS - 1) / SUBS; turns > 0; --turns, n += SUBS) {
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      x[k] = x1[k];
+      if constexpr (BWD) e[k] = e1[k];
+    }
+    const T mean = mean1, rstd = rstd1;
+    if (turns > 1) fetch_next(n + SUBS);
+    const int64_t at = n * p.C + g * p.m;
+    if constexpr (!BWD) {
+      double2 t = make_double2(0.0, 0.0);
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) t.x += (double)x[k].v[i];
+      const double mu = row_sum<LANES>(t).x / count;
+      // The mean in two parts: x - high is exact near the mean.
+      const T high = (T)mu, low = (T)(mu - (double)high);
+      t.x = 0.0;
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          x[k].v[i] = (x[k].v[i] - high) - low;
+          if (on[k]) t.x = fma((double)x[k].v[i], (double)x[k].v[i], t.x);
+        }
+      const double r64 = 1.0 / sqrt(row_sum<LANES>(t).x / count + p.eps);
+      const T r = (T)r64;
+      if (n < n1) {
+        if (lane == 0) {
+          if (p.mean) p.mean[n * p.G + g] = (T)mu;
+          if (p.rstd) p.rstd[n * p.G + g] = r;
+        }
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+          if (!on[k]) continue;
+          Pack<T, V> o;
+#pragma unroll
+          for (int i = 0; i < V; ++i) o.v[i] = activate(act, fma(x[k].v[i] * r, w[k][i], b[k][i]));
+          store_pack<T, V>(p.out + at + (k * LANES + lane) * V, o);
+        }
+      }
+    } else {
+      // x becomes xhat, e becomes w dz.
+      double2 t = make_double2(0.0, 0.0);
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) {
+        if (!on[k] || n >= n1) continue;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const T xh = (x[k].v[i] - mean) * rstd;
+          const T dz = e[k].v[i] * slope(act, fma(xh, w[k][i], b[k][i]));
+          const T prod = dz * xh;
+          db[k][i] += (double)dz;
+          dw[k][i] += (double)prod;
+          t.x = fma((double)w[k][i], (double)dz, t.x);
+          t.y = fma((double)w[k][i], (double)prod, t.y);
+          x[k].v[i] = xh;
+          e[k].v[i] = dz;
+        }
+      }
+      t = row_sum<LANES>(t);
+      const T m1 = (T)(t.x / count), m2 = (T)(t.y / count);
+      if (n < n1) {
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+          if (!on[k]) continue;
+          Pack<T, V> o;
+#pragma unroll
+          for (int i = 0; i < V; ++i) o.v[i] = rstd * (fma(w[k][i], e[k].v[i], -m1) - x[k].v[i] * m2);
+          store_pack<T, V>(p.out + at + (k * LANES + lane) * V, o);
+        }
+      }
+    }
+  }
+  if constexpr (BWD) {
+    if (!p.part) return;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        double2 t = make_double2(db[k][i], dw[k][i]);
+#pragma unroll
+        for (int o = LANES; o < UNIT; o <<= 1) {
+          t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
+          t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
+        }
+        if (on[k] && sub == 0) p.part[chunk * p.C + g * p.m + (k * LANES + lane) * V + i] = t;
+      }
+  }
+}
+
+// dweight and dbias: `rows` rows of per-channel sums, added in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) norm_affine_kernel(const double2* sums, int64_t rows, int64_t C, T* dweight,
+                                                               T* dbias) {
+  __shared__ double2 red[kWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  double2 t = make_double2(0.0, 0.0);
+  if (c < C) {
+#pragma unroll 4
+    for (int64_t r = warp; r < rows; r += kWarps) {
+      const double2 v = sums[r * C + c];
+      t.x += v.x;
+      t.y += v.y;
+    }
+  }
+  red[warp][lane] = t;
+  __syncthreads();
+  if (warp == 0 && c < C) {
+    for (int w = 1; w < kWarps; ++w) {
+      t.x += red[w][lane].x;
+      t.y += red[w][lane].y;
+    }
+    if (dbias) dbias[c] = (T)t.x;
+    if (dweight) dweight[c] = (T)t.y;
+  }
+}
+
+template <typename T>
+int launch_affine(Device* d, const double2* sums, int64_t rows, const NormArgs<T>& p) {
+  const int64_t blocks = ceil_div(p.C, (int64_t)32);
+  if (blocks > INT32_MAX) PB_FAIL(PB_ERR_UNSUPPORTED, "too many channels");
+  norm_affine_kernel<T><<<(unsigned)blocks, kThreads, 0, d->stream>>>(sums, rows, p.C, p.dweight, p.dbias);
+  PB_LAUNCHED(d);
+  return PB_OK;
+}
+
+template <typename T, int V, int LANES, int ITEMS, bool BWD>
+int launch_rows(Device* d, int act, NormArgs<T> p) {
+  constexpr int UNIT = LANES < 32 ? 32 : LANES, SUBS = UNIT / LANES;
+  const void* kernel = (const void*)norm_rows_kernel<T, V, LANES, ITEMS, BWD>;
+  // One wave of units, each at least one row per part (backward: 16, so that
+  // the sums it writes are little beside what it reads).
+  const int64_t wave = resident_blocks(d, kernel, kThreads) * (kThreads / UNIT);
+  int64_t chunks = ceil_div(wave, p.G);
+  const bool sums = BWD && (p.dweight || p.dbias);
+  const int64_t most = ceil_div(p.N, (int64_t)SUBS * (sums ? 16 : 1));
+  if (chunks > most) chunks = most;
+  p.rows = ceil_div(p.N, chunks);
+  p.chunks = ceil_div(p.N, p.rows);
+  p.part = nullptr;
+  if (sums) {
+    size_t bytes;
+    const int64_t e[] = {p.chunks, p.C};
+    if (!array_bytes(e, 2, sizeof(double2), &bytes)) PB_FAIL(PB_ERR_INVALID, "extents too large");
+    void* ws;
+    PB_CHECK(scratch(d, bytes, &ws));
+    p.part = static_cast<double2*>(ws);
+  }
+  const int64_t blocks = ceil_div(p.G * p.chunks, (int64_t)(kThreads / UNIT));
+  if (blocks > INT32_MAX) PB_FAIL(PB_ERR_UNSUPPORTED, "too many groups");
+  PB_CHECK(kt_begin(d));
+  norm_rows_kernel<T, V, LANES, ITEMS, BWD><<<(unsigned)blocks, kThreads, 0, d->stream>>>(p, act);
+  PB_LAUNCHED(d);
+  PB_CHECK(kt_end(d));
+  return sums ? launch_affine<T>(d, p.part, p.chunks, p) : PB_OK;
+}
+
+// Whether rows of m values fit the rows kernel: 1024 packs at most.
+constexpr int64_t kRowPacks = 1024;
+
+template <typename T, int V, bool BWD>
+int launch_rows_of(Device* d, int act, const NormArgs<T>& p) {
+  const int64_t packs = ceil_div(p.m, (int64_t)V);
+  if (packs <= 8) return launch_rows<T, V, 8, 1, BWD>(d, act, p);
+  if (packs <= 16) return launch_rows<T, V, 8, 2, BWD>(d, act, p);
+  if (packs <= 32) return launch_rows<T, V, 16, 2, BWD>(d, act, p);
+  if (packs <= 64) return launch_rows<T, V, 32, 2, BWD>(d, act, p);
+  if (packs <= 128) return launch_rows<T, V, 32, 4, BWD>(d, act, p);
+  if (packs <= 256) return launch_rows<T, V, 256, 1, BWD>(d, act, p);
+  if (packs <= 512) return launch_rows<T, V, 256, 2, BWD>(d, act, p);
+  return launch_rows<T, V, 256, 4, BWD>(d, act, p);
 }
 
 template <typename T, int V, int ACT, bool BWD>
@@ -290,8 +547,7 @@ int launch(Device* d, NormArgs<T> p) {
   PB_LAUNCHED(d);
   PB_CHECK(kt_end(d));
   if (BWD && (p.dweight || p.dbias)) {
-    norm_affine_kernel<T><<<(unsigned)ceil_div(p.C, (int64_t)kThreads), kThreads, 0, d->stream>>>(p);
-    PB_LAUNCHED(d);
+    return launch_affine<T>(d, p.chan, p.N, p);
   }
   return PB_OK;
 }
@@ -331,6 +587,8 @@ int dispatch(Device* d, int act, int64_t N, int64_t S, int64_t C, int64_t G, dou
   p.eps = eps;
   constexpr int V = Vec16<T>::n;
   const bool wide = C % V == 0 && (((uintptr_t)q.x | (uintptr_t)q.dy | (uintptr_t)q.out) & 15) == 0;
+  if (S == 1 && p.m <= kRowPacks * (wide && p.m % V == 0 ? V : 1))
+    return wide && p.m % V == 0 ? launch_rows_of<T, V, BWD>(d, act, p) : launch_rows_of<T, 1, BWD>(d, act, p);
   return wide ? launch_act<T, V, BWD>(d, act, p) : launch_act<T, 1, BWD>(d, act, p);
 }
 
