@@ -4,14 +4,17 @@
 // x is (N, S, C), C = G groups of m channels; a group's set is its m channels
 // over the S positions of one sample.  Channels are contiguous, so lanes run
 // over channels and every sum over positions is a sum down a column:
-//   sums   each block takes a run of positions of one sample and adds up two
-//          numbers per channel in float64 (forward: x - k and (x - k)^2 with
-//          the shift k = the group's first value, which keeps the variance of
-//          values far from zero; backward: dz and dz * xhat).  The block that
-//          finishes a sample last adds the blocks' sums in block order and then
-//          the channels of each group, so the result is deterministic.
-//   apply  a second pass over the same positions.
-// The second read comes from L2 while a sample is still there.
+//   sums   adds up two numbers per channel in float64 over a run of positions of
+//          one sample (forward: x - k and (x - k)^2 with the shift k = the group's
+//          first value, which keeps the variance of values far from zero;
+//          backward: dz and dz * xhat), then over the channels of each group.  The
+//          block that finishes a sample last adds its runs' sums in a fixed
+//          order, so the result is deterministic.
+//   apply  reads the run again and writes the result.
+// One launch does both: resident blocks take sums and apply items from a counter
+// whose order interleaves them, a sample's apply items following its sums by
+// about one item per block.  The second read then finds the sample in L2
+// (up to about half of its 126 MB) while the next sample's first read keeps HBM busy.
 //
 // With one position (S = 1: a norm of each token) a group is a row of m
 // contiguous values, which fits into the registers of a part of a warp, a warp
@@ -32,13 +35,16 @@ struct NormArgs {
   T* out;             // y or dx
   T *mean, *rstd;     // forward: outputs, may be null; backward: inputs
   T *dweight, *dbias; // may be null
-  double2* part;      // (N, chunks, C): per-channel sums of a block
-  double2* chan;      // (N, C): per-channel sums of a sample
+  double2* chan;      // per-channel sums of each (n, chunk): backward, and forward beyond kSharedChannels
+  double2* part;      // (N, chunks, G): per-group sums
   double2* group;     // (N, G): forward (mean, rstd); backward (mean of w dz, mean of w dz xhat)
+  unsigned* words;    // see pb_layers.cuh: a flag per sample
+  int* err;
   unsigned* arrivals; // N words, zero on entry and exit
   int64_t N, S, C, G, m;
-  int64_t rows;       // positions per block
-  int64_t chunks;     // blocks per sample
+  int64_t rows;       // positions per item
+  int64_t chunks;     // items per sample
+  FastDiv by_chunks, by_m;
   double eps;
 };
 
@@ -83,102 +89,118 @@ __device__ __forceinline__ double shift_of(const NormArgs<T>& p, int64_t n, int6
   return isfinite(k) ? k : 0.0;
 }
 
-// Sums pass.  Threads form tx lanes over packs of V channels and ty rows.
+// Channels whose sums a block holds in shared memory.
+constexpr int64_t kSharedChannels = 1024;
+
+// The group sums of one item: threads form tx lanes over packs of V channels
+// and ty rows.
 template <typename T, int V, int ACT, bool BWD>
-__global__ void __launch_bounds__(kThreads) norm_sums_kernel(const NormArgs<T> p, int tx, int ty) {
-  __shared__ double2 red[kThreads];
-  __shared__ bool last;
+__device__ __forceinline__ void sums_item(const NormArgs<T>& p, int64_t unit, int tx, int ty, double2* red, double2* shared) {
   const int lx = threadIdx.x % tx, ly = threadIdx.x / tx;
-  for (int64_t unit = blockIdx.x; unit < p.N * p.chunks; unit += gridDim.x) {
-    const int64_t n = unit / p.chunks, chunk = unit % p.chunks;
-    const int64_t r0 = chunk * p.rows, r1 = min(p.S, r0 + p.rows);
-    double2* const part = p.part + unit * p.C;
-    for (int64_t c0 = 0; c0 < p.C; c0 += (int64_t)tx * V) {
-      const int64_t c = c0 + (int64_t)lx * V;
-      const bool on = ly < ty && c < p.C;
-      double s1[V] = {}, s2[V] = {};
-      if (on) {
-        double k[V];
-        T mean[V], rstd[V], w[V], b[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int64_t g = (c + i) / p.m;
-          if constexpr (BWD) {
-            mean[i] = __ldg(p.mean + n * p.G + g);
-            rstd[i] = __ldg(p.rstd + n * p.G + g);
-            w[i] = p.weight ? __ldg(p.weight + c + i) : T(1);
-            b[i] = p.bias ? __ldg(p.bias + c + i) : T(0);
-          } else {
-            k[i] = shift_of(p, n, g);
-          }
-        }
-        const T* x = p.x + (n * p.S + r0 + ly) * p.C + c;
-        const T* dy = BWD ? p.dy + (n * p.S + r0 + ly) * p.C + c : nullptr;
-#pragma unroll 4
-        for (int64_t r = r0 + ly; r < r1; r += ty) {
-          const Pack<T, V> q = load_pack<T, V>(x);
-          x += ty * p.C;
-          if constexpr (BWD) {
-            const Pack<T, V> e = load_pack<T, V>(dy);
-            dy += ty * p.C;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const T xh = (q.v[i] - mean[i]) * rstd[i];
-              const T dz = e.v[i] * slope<T, ACT>(fma(xh, w[i], b[i]));
-              s1[i] += (double)dz;
-              s2[i] += (double)(dz * xh);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const double v = (double)q.v[i] - k[i];
-              s1[i] += v;
-              s2[i] = fma(v, v, s2[i]);
-            }
-          }
-        }
-      }
+  const int64_t n = fdiv(unit, p.by_chunks), chunk = unit - n * p.chunks;
+  const int64_t r0 = chunk * p.rows, r1 = min(p.S, r0 + p.rows);
+  double2* const out = p.C <= kSharedChannels ? shared : p.chan + unit * p.C;
+  for (int64_t c0 = 0; c0 < p.C; c0 += (int64_t)tx * V) {
+    const int64_t c = c0 + (int64_t)lx * V;
+    const bool on = ly < ty && c < p.C;
+    double s1[V] = {}, s2[V] = {};
+    if (on) {
+      double k[V];
+      T mean[V], rstd[V], w[V], b[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        __syncthreads();
-        red[threadIdx.x] = make_double2(s1[i], s2[i]);
-        __syncthreads();
-        if (on && ly == 0) {
-          double2 t = red[lx];
-          for (int y = 1; y < ty; ++y) {
-            t.x += red[y * tx + lx].x;
-            t.y += red[y * tx + lx].y;
+        const int64_t g = fdiv(c + i, p.by_m);
+        if constexpr (BWD) {
+          mean[i] = __ldg(p.mean + n * p.G + g);
+          rstd[i] = __ldg(p.rstd + n * p.G + g);
+          w[i] = p.weight ? __ldg(p.weight + c + i) : T(1);
+          b[i] = p.bias ? __ldg(p.bias + c + i) : T(0);
+        } else {
+          k[i] = shift_of(p, n, g);
+        }
+      }
+      const T* x = p.x + (n * p.S + r0 + ly) * p.C + c;
+      const T* dy = BWD ? p.dy + (n * p.S + r0 + ly) * p.C + c : nullptr;
+#pragma unroll 4
+      for (int64_t r = r0 + ly; r < r1; r += ty) {
+        const Pack<T, V> q = load_pack<T, V>(x);
+        x += ty * p.C;
+        if constexpr (BWD) {
+          const Pack<T, V> e = load_pack<T, V>(dy);
+          dy += ty * p.C;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const T xh = (q.v[i] - mean[i]) * rstd[i];
+            const T dz = e.v[i] * slope<T, ACT>(fma(xh, w[i], b[i]));
+            s1[i] += (double)dz;
+            s2[i] += (double)(dz * xh);
           }
-          part[c + i] = t;
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const double v = (double)q.v[i] - k[i];
+            s1[i] += v;
+            s2[i] = fma(v, v, s2[i]);
+          }
         }
       }
     }
-    // The last block of the sample adds up the blocks' sums.
-    __threadfence();
+    // Over the rows of threads, in row order.
+#pragma unroll
+    for (int i = 0; i < V; ++i) red[i * kThreads + threadIdx.x] = make_double2(s1[i], s2[i]);
     __syncthreads();
-    if (threadIdx.x == 0) last = p.chunks == 1 || atomicAdd(&p.arrivals[n], 1u) == (unsigned)p.chunks - 1;
+    for (int q = threadIdx.x; q < tx * V; q += kThreads) {
+      const int i = q % V, l = q / V;
+      if (c0 + q >= p.C) break;
+      double2 t = red[i * kThreads + l];
+      for (int y = 1; y < ty; ++y) {
+        t.x += red[i * kThreads + y * tx + l].x;
+        t.y += red[i * kThreads + y * tx + l].y;
+      }
+      out[c0 + q] = t;
+      if (BWD && out == shared && p.chan) p.chan[unit * p.C + c0 + q] = t;
+    }
     __syncthreads();
-    if (!last) continue;
-    __threadfence();
-    for (int64_t c = threadIdx.x; c < p.C; c += kThreads) {
-      double2 t = make_double2(0.0, 0.0);
-      const double2* q = p.part + n * p.chunks * p.C + c;
-      for (int64_t k = 0; k < p.chunks; ++k, q += p.C) {
+  }
+  // Over the channels of each group.
+  for (int64_t g = threadIdx.x; g < p.G; g += kThreads) {
+    double2 t = make_double2(0.0, 0.0);
+    for (int64_t c = g * p.m; c < (g + 1) * p.m; ++c) {
+      const double2 v = out[c];
+      const double w = BWD && p.weight ? (double)__ldg(p.weight + c) : 1.0;
+      t.x = fma(w, v.x, t.x);
+      t.y = fma(w, v.y, t.y);
+    }
+    p.part[unit * p.G + g] = t;
+  }
+}
+
+// The statistics of a sample from its items' group sums.  The threads take
+// (group, every lanes-th item) and meet in shared memory.
+template <typename T, bool BWD>
+__device__ __forceinline__ void merge_sample(const NormArgs<T>& p, int64_t n, double2* red) {
+  const int wide = p.G < kThreads ? (int)p.G : kThreads, lanes = kThreads / wide;
+  const int lg = threadIdx.x % wide, lk = threadIdx.x / wide;
+  const double count = (double)p.S * (double)p.m;
+  for (int64_t g0 = 0; g0 < p.G; g0 += wide) {
+    const int64_t g = g0 + lg;
+    double2 t = make_double2(0.0, 0.0);
+    if (g < p.G && lk < lanes) {
+      const double2* q = p.part + (n * p.chunks + lk) * p.G + g;
+#pragma unroll 4
+      for (int64_t k = lk; k < p.chunks; k += lanes, q += (int64_t)lanes * p.G) {
         const double2 v = __ldcg(q);
         t.x += v.x;
         t.y += v.y;
       }
-      p.chan[n * p.C + c] = t;
     }
     __syncthreads();
-    const double count = (double)p.S * (double)p.m;
-    for (int64_t g = threadIdx.x; g < p.G; g += kThreads) {
-      double2 t = make_double2(0.0, 0.0);
-      for (int64_t c = g * p.m; c < (g + 1) * p.m; ++c) {
-        const double2 v = p.chan[n * p.C + c];
-        const double w = BWD && p.weight ? (double)__ldg(p.weight + c) : 1.0;
-        t.x = fma(w, v.x, t.x);
-        t.y = fma(w, v.y, t.y);
+    red[threadIdx.x] = t;
+    __syncthreads();
+    if (lk == 0 && g < p.G) {
+      for (int k = 1; k < lanes; ++k) {
+        t.x += red[k * wide + lg].x;
+        t.y += red[k * wide + lg].y;
       }
       t.x /= count;
       t.y /= count;
@@ -193,62 +215,111 @@ __global__ void __launch_bounds__(kThreads) norm_sums_kernel(const NormArgs<T> p
       }
       p.group[n * p.G + g] = t;
     }
-    if (threadIdx.x == 0 && p.chunks > 1) p.arrivals[n] = 0;
-    __syncthreads();
   }
 }
 
 template <typename T, int V, int ACT, bool BWD>
-__global__ void __launch_bounds__(kThreads) norm_apply_kernel(const NormArgs<T> p, int tx, int ty) {
+__device__ __forceinline__ void apply_item(const NormArgs<T>& p, int64_t unit, int tx, int ty) {
   const int lx = threadIdx.x % tx, ly = threadIdx.x / tx;
-  for (int64_t unit = blockIdx.x; unit < p.N * p.chunks; unit += gridDim.x) {
-    const int64_t n = unit / p.chunks, chunk = unit % p.chunks;
-    const int64_t r0 = chunk * p.rows, r1 = min(p.S, r0 + p.rows);
-    for (int64_t c = (int64_t)lx * V; c < p.C && ly < ty; c += (int64_t)tx * V) {
-      T mean[V], low[V], rstd[V], w[V], b[V], m1[V], m2[V];
+  const int64_t n = fdiv(unit, p.by_chunks), chunk = unit - n * p.chunks;
+  const int64_t r0 = chunk * p.rows, r1 = min(p.S, r0 + p.rows);
+  for (int64_t c = (int64_t)lx * V; c < p.C && ly < ty; c += (int64_t)tx * V) {
+    T mean[V], low[V], rstd[V], w[V], b[V], m1[V], m2[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int64_t g = (c + i) / p.m;
-        const double2 t = p.group[n * p.G + g];
-        w[i] = p.weight ? __ldg(p.weight + c + i) : T(1);
-        b[i] = p.bias ? __ldg(p.bias + c + i) : T(0);
-        if constexpr (BWD) {
-          mean[i] = __ldg(p.mean + n * p.G + g);
-          rstd[i] = __ldg(p.rstd + n * p.G + g);
-          m1[i] = (T)t.x;
-          m2[i] = (T)t.y;
-        } else {
-          // The mean in two parts, so that its rounding does not show where
-          // the values lie far from zero.
-          mean[i] = (T)t.x;
-          low[i] = (T)(t.x - (double)mean[i]);
-          rstd[i] = (T)t.y;
-        }
-      }
-      int64_t at = (n * p.S + r0 + ly) * p.C + c;
-#pragma unroll 4
-      for (int64_t r = r0 + ly; r < r1; r += ty, at += ty * p.C) {
-        const Pack<T, V> q = load_pack<T, V>(p.x + at);
-        Pack<T, V> o;
-        if constexpr (BWD) {
-          const Pack<T, V> e = load_pack<T, V>(p.dy + at);
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const T xh = (q.v[i] - mean[i]) * rstd[i];
-            const T dz = e.v[i] * slope<T, ACT>(fma(xh, w[i], b[i]));
-            o.v[i] = rstd[i] * (fma(w[i], dz, -m1[i]) - xh * m2[i]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const T xh = ((q.v[i] - mean[i]) - low[i]) * rstd[i];
-            o.v[i] = activate<T, ACT>(fma(xh, w[i], b[i]));
-          }
-        }
-        store_pack<T, V>(p.out + at, o);
+    for (int i = 0; i < V; ++i) {
+      const int64_t g = fdiv(c + i, p.by_m);
+      const double2 t = __ldcg(p.group + n * p.G + g);
+      w[i] = p.weight ? __ldg(p.weight + c + i) : T(1);
+      b[i] = p.bias ? __ldg(p.bias + c + i) : T(0);
+      if constexpr (BWD) {
+        mean[i] = __ldg(p.mean + n * p.G + g);
+        rstd[i] = __ldg(p.rstd + n * p.G + g);
+        m1[i] = (T)t.x;
+        m2[i] = (T)t.y;
+      } else {
+        // The mean in two parts, so that its rounding does not show where
+        // the values lie far from zero.
+        mean[i] = (T)t.x;
+        low[i] = (T)(t.x - (double)mean[i]);
+        rstd[i] = (T)t.y;
       }
     }
+    int64_t at = (n * p.S + r0 + ly) * p.C + c;
+#pragma unroll 4
+    for (int64_t r = r0 + ly; r < r1; r += ty, at += ty * p.C) {
+      const Pack<T, V> q = load_pack<T, V>(p.x + at);
+      Pack<T, V> o;
+      if constexpr (BWD) {
+        const Pack<T, V> e = load_pack<T, V>(p.dy + at);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const T xh = (q.v[i] - mean[i]) * rstd[i];
+          const T dz = e.v[i] * slope<T, ACT>(fma(xh, w[i], b[i]));
+          o.v[i] = rstd[i] * (fma(w[i], dz, -m1[i]) - xh * m2[i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const T xh = ((q.v[i] - mean[i]) - low[i]) * rstd[i];
+          o.v[i] = activate<T, ACT>(fma(xh, w[i], b[i]));
+        }
+      }
+      store_pack<T, V>(p.out + at, o);
+    }
   }
+}
+
+// Items in the order of their numbers: `lead` sums, then apply and sums in
+// turn, then the rest of apply.  lead is a sample's items and one per block, so
+// apply item j comes behind all sums of its sample.
+template <typename T, int V, int ACT, bool BWD>
+__global__ void __launch_bounds__(kThreads, 2) norm_samples_kernel(const NormArgs<T> p, int tx, int ty, unsigned units,
+                                                                   unsigned lead) {
+  __shared__ double2 red[kThreads * V];
+  __shared__ double2 channels[kSharedChannels];
+  __shared__ unsigned item_s, epoch_s;
+  __shared__ bool last;
+  if (threadIdx.x == 0) {
+    item_s = atomicAdd(p.words, 1u);
+    epoch_s = load_acquire(p.words + 2) + 1;
+  }
+  __syncthreads();
+  const unsigned epoch = epoch_s;
+  for (unsigned item = item_s; item < 2 * units; item = item_s) {
+    const unsigned turn = item - lead;  // used from item `lead` on
+    bool sums;
+    unsigned unit;
+    if (item < lead) sums = true, unit = item;
+    else if (turn < 2 * (units - lead)) sums = turn & 1u, unit = turn / 2 + (sums ? lead : 0u);
+    else sums = false, unit = turn - (units - lead);
+    const int64_t n = fdiv(unit, p.by_chunks);
+    if (sums) {
+      sums_item<T, V, ACT, BWD>(p, unit, tx, ty, red, channels);
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0)
+        last = p.chunks == 1 || atomicAdd(&p.arrivals[n], 1u) == (unsigned)p.chunks - 1;
+      __syncthreads();
+      if (last) {
+        __threadfence();
+        merge_sample<T, BWD>(p, n, red);
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          if (p.chunks > 1) p.arrivals[n] = 0;
+          store_release(p.words + kFlagWords + n, epoch);
+        }
+      }
+    } else {
+      if (threadIdx.x == 0) wait_flag(p.words + kFlagWords + n, epoch, p.err);
+      __syncthreads();
+      apply_item<T, V, ACT, BWD>(p, unit, tx, ty);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) item_s = atomicAdd(p.words, 1u);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) finish_words(p.words, epoch, gridDim.x);
 }
 
 template <typename T>
@@ -521,35 +592,41 @@ template <typename T, int V, int ACT, bool BWD>
 int launch(Device* d, NormArgs<T> p) {
   const int64_t lanes = ceil_div(p.C, (int64_t)V);
   const int tx = (int)(lanes < kThreads ? lanes : kThreads), ty = kThreads / tx;
-  // Blocks of at least 16 positions per thread, about eight per SM in all.
-  int64_t chunks = ceil_div((int64_t)d->sm_count * 8, p.N);
-  const int64_t most = ceil_div(p.S, (int64_t)ty * 16);
+  const void* kernel = (const void*)norm_samples_kernel<T, V, ACT, BWD>;
+  const int64_t wave = resident_blocks(d, kernel, kThreads);
+  // About four items per block and pass, each at least four positions per thread.
+  int64_t chunks = ceil_div(wave * 4, p.N);
+  const int64_t most = ceil_div(p.S, (int64_t)ty * 4);
   if (chunks > most) chunks = most;
   p.rows = ceil_div(p.S, chunks);
   p.chunks = ceil_div(p.S, p.rows);
-  size_t part, chan, group;
-  const int64_t e1[] = {p.N, p.chunks, p.C}, e2[] = {p.N, p.C}, e3[] = {p.N, p.G};
-  if (!array_bytes(e1, 3, sizeof(double2), &part) || !array_bytes(e2, 2, sizeof(double2), &chan) ||
+  p.by_chunks = make_fastdiv(p.chunks);
+  p.by_m = make_fastdiv(p.m);
+  const int64_t units = p.N * p.chunks;
+  if (units >= (int64_t(1) << 30)) PB_FAIL(PB_ERR_UNSUPPORTED, "more than 2^30 samples");
+  const bool affine = BWD && (p.dweight || p.dbias);
+  const bool by_channel = affine || p.C > kSharedChannels;
+  size_t chan = 0, part, group;
+  const int64_t e1[] = {units, p.C}, e2[] = {units, p.G}, e3[] = {p.N, p.G};
+  if ((by_channel && !array_bytes(e1, 2, sizeof(double2), &chan)) || !array_bytes(e2, 2, sizeof(double2), &part) ||
       !array_bytes(e3, 2, sizeof(double2), &group))
     PB_FAIL(PB_ERR_INVALID, "extents too large");
   void* ws;
   PB_CHECK(scratch(d, part + chan + group, &ws));
   p.part = static_cast<double2*>(ws);
-  p.chan = p.part + part / sizeof(double2);
-  p.group = p.chan + chan / sizeof(double2);
+  p.group = p.part + part / sizeof(double2);
+  p.chan = by_channel ? p.group + group / sizeof(double2) : nullptr;
   if (p.chunks > 1) PB_CHECK(counters(d, (size_t)p.N, &p.arrivals));
-  const int64_t units = p.N * p.chunks, cap = int64_t(1) << 30;
-  const unsigned grid = (unsigned)(units < cap ? units : cap);
+  PB_CHECK(epoch_words(d, kFlagWords + (size_t)p.N, &p.words));
+  p.err = d->err_dev;
+  const int64_t grid = 2 * units < wave ? 2 * units : wave;
+  const int64_t lead = p.chunks + grid < units ? p.chunks + grid : units;
   PB_CHECK(kt_begin(d));
-  norm_sums_kernel<T, V, ACT, BWD><<<grid, kThreads, 0, d->stream>>>(p, tx, ty);
-  PB_LAUNCHED(d);
-  norm_apply_kernel<T, V, ACT, BWD><<<grid, kThreads, 0, d->stream>>>(p, tx, ty);
+  norm_samples_kernel<T, V, ACT, BWD>
+      <<<(unsigned)grid, kThreads, 0, d->stream>>>(p, tx, ty, (unsigned)units, (unsigned)lead);
   PB_LAUNCHED(d);
   PB_CHECK(kt_end(d));
-  if (BWD && (p.dweight || p.dbias)) {
-    return launch_affine<T>(d, p.chan, p.N, p);
-  }
-  return PB_OK;
+  return affine ? launch_affine<T>(d, p.chan, units, p) : PB_OK;
 }
 
 template <typename T, int V, bool BWD>

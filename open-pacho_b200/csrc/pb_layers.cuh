@@ -59,6 +59,50 @@ __device__ __forceinline__ void sigmoid_pair(T z, T* s, T* rest) {
   *rest = neg ? big : small;
 }
 
+// ---- flags between the blocks of one launch (words of epoch_words()) ----
+//
+// words[0] counts the work items handed out, words[1] the blocks that are done,
+// words[2] is the number of launches so far; flags follow from kFlagWords on.
+// An item waits only for flags of items with lower numbers, which are running or
+// done when it gets its own, so every wait ends.
+constexpr int kFlagWords = 4;
+constexpr unsigned long long kFlagWaitNs = 4ull * 1000 * 1000 * 1000;
+
+__device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
+  unsigned v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_release(unsigned* p, unsigned v) {
+  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+// Wait for a flag of this launch; after kFlagWaitNs the error word is set and the
+// kernel goes on to its end (with wrong values).
+__device__ __forceinline__ void wait_flag(const unsigned* flag, unsigned epoch, int* err) {
+  if (load_acquire(flag) == epoch) return;
+  unsigned long long t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  while (load_acquire(flag) != epoch) {
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    if (t - t0 > kFlagWaitNs) {
+      atomicExch(err, KERR_WAIT_TIMEOUT);
+      return;
+    }
+  }
+}
+
+// The last block to finish readies the words for the next launch: flags need no
+// clearing, the next epoch's value is another.  One thread of each block, after
+// the block's last use of the words.
+__device__ __forceinline__ void finish_words(unsigned* words, unsigned epoch, unsigned blocks) {
+  __threadfence();
+  if (atomicAdd(words + 1, 1u) == blocks - 1) {
+    words[0] = 0;
+    words[1] = 0;
+    words[2] = epoch;
+  }
+}
+
 // Whether [p, p + pn) and [q, q + qn) share a byte (NULL shares none).
 inline bool overlap(const void* p, size_t pn, const void* q, size_t qn) {
   const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;

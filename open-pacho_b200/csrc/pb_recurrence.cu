@@ -33,7 +33,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kGroup = 16;  // chunks per group
-constexpr unsigned long long kWaitNs = 4ull * 1000 * 1000 * 1000;
 
 template <typename T>
 struct ScanArgs {
@@ -201,29 +200,6 @@ __device__ __forceinline__ double2 compose(const double2& a, const double2& b) {
   return make_double2(a.x * b.x, apply(b, a.y));
 }
 
-__device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
-  unsigned v;
-  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ void store_release(unsigned* p, unsigned v) {
-  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
-}
-// Wait for a flag of this launch; after kWaitNs the error word is set and the
-// kernel goes on to its end (with wrong values).
-__device__ __forceinline__ void wait_flag(const unsigned* flag, unsigned epoch, int* err) {
-  if (load_acquire(flag) == epoch) return;
-  unsigned long long t0, t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  while (load_acquire(flag) != epoch) {
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (t - t0 > kWaitNs) {
-      atomicExch(err, KERR_WAIT_TIMEOUT);
-      return;
-    }
-  }
-}
-
 // One block per (column tile, chunk).  A warp covers 2^lanes_log2 columns and
 // 32 >> lanes_log2 consecutive pieces of L steps, the block kWarps times that.
 // Blocks take their chunk from a counter, chunk by chunk over the column
@@ -280,8 +256,8 @@ __global__ void __launch_bounds__(kThreads, BWD ? (sizeof(T) == 4 ? 3 : 2) : 4) 
   __syncthreads();
 
   const unsigned groups = (p.chunks + kGroup - 1) / kGroup;
-  unsigned* const chunk_flag = p.words + 4 + (size_t)tile * p.chunks;
-  unsigned* const group_flag = p.words + 4 + (size_t)p.tiles * p.chunks + (size_t)tile * groups;
+  unsigned* const chunk_flag = p.words + kFlagWords + (size_t)tile * p.chunks;
+  unsigned* const group_flag = p.words + kFlagWords + (size_t)p.tiles * p.chunks + (size_t)tile * groups;
   const unsigned group = chunk / kGroup, place = chunk % kGroup;
   const bool behind = chunk + 1 < p.chunks;  // some chunk waits for this one
   const bool writer = piece == 0 && on;
@@ -331,16 +307,7 @@ __global__ void __launch_bounds__(kThreads, BWD ? (sizeof(T) == 4 ? 3 : 2) : 4) 
   x = apply(before, x);
   if (on && s0 < p.length) st.run(p, base, col, s0, (T)x);
 
-  // The last block to finish readies the words for the next launch: flags
-  // need no clearing, the next epoch's value is another.
-  if (threadIdx.x == 0) {
-    __threadfence();
-    if (atomicAdd(p.words + 1, 1u) == p.tiles * p.chunks - 1) {
-      p.words[0] = 0;
-      p.words[1] = 0;
-      p.words[2] = epoch;
-    }
-  }
+  if (threadIdx.x == 0) finish_words(p.words, epoch, p.tiles * p.chunks);
 }
 
 template <typename T, int GATE, bool BWD>
@@ -360,7 +327,7 @@ int launch(Device* d, ScanArgs<T>& p) {
     PB_CHECK(scratch(d, maps * sizeof(double2) + ends * sizeof(double), &ws));
     p.maps = static_cast<double2*>(ws);
     p.ends = reinterpret_cast<double*>(p.maps + maps);
-    PB_CHECK(epoch_words(d, 4 + (size_t)(tiles * (chunks + groups)), &p.words));
+    PB_CHECK(epoch_words(d, kFlagWords + (size_t)(tiles * (chunks + groups)), &p.words));
     p.lanes_log2 = lanes;
     p.tiles = (unsigned)tiles;
     p.chunks = (unsigned)chunks;
