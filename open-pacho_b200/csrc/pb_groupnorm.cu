@@ -51,11 +51,7 @@ struct NormArgs {
 template <typename T, int ACT>
 __device__ __forceinline__ T activate(T z) {
   if constexpr (ACT == PB_ACT_RELU) return z < T(0) ? T(0) : z;
-  if constexpr (ACT == PB_ACT_SILU) {
-    T s, rest;
-    sigmoid_pair(z, &s, &rest);
-    return z * s;
-  }
+  if constexpr (ACT == PB_ACT_SILU) return z * sigmoid(z);
   if constexpr (ACT == PB_ACT_GELU) {
     // z Phi(z) with Phi(z) = erfc(-z / sqrt 2) / 2, which keeps its relative
     // accuracy for negative z where 1 + erf would cancel.
@@ -69,9 +65,8 @@ template <typename T, int ACT>
 __device__ __forceinline__ T slope(T z) {
   if constexpr (ACT == PB_ACT_RELU) return z > T(0) ? T(1) : T(0);
   if constexpr (ACT == PB_ACT_SILU) {
-    T s, rest;
-    sigmoid_pair(z, &s, &rest);
-    return s * fma(z, rest, T(1));
+    const T s = sigmoid(z);
+    return fma(s * z, T(1) - s, s);
   }
   if constexpr (ACT == PB_ACT_GELU) {
     const T phi = exp_of(T(-0.5) * z * z) * T(0.39894228040143268);
@@ -270,10 +265,17 @@ __device__ __forceinline__ void apply_item(const NormArgs<T>& p, int64_t unit, i
 }
 
 // Items in the order of their numbers: `lead` sums, then apply and sums in
-// turn, then the rest of apply.  lead is a sample's items and one per block, so
-// apply item j comes behind all sums of its sample.
+// turn, then the rest of apply.  lead is a sample's items and two per block (the
+// one it works on and the one it holds), so apply item j comes behind all sums of its
+// sample.
+#ifndef PB_ITEMS
+#define PB_ITEMS 2
+#define PB_ROWS 64
+#define PB_FB 3
+#define PB_BB 2
+#endif
 template <typename T, int V, int ACT, bool BWD>
-__global__ void __launch_bounds__(kThreads, 2) norm_samples_kernel(const NormArgs<T> p, int tx, int ty, unsigned units,
+__global__ void __launch_bounds__(kThreads, BWD ? PB_BB : PB_FB) norm_samples_kernel(const NormArgs<T> p, int tx, int ty, unsigned units,
                                                                    unsigned lead) {
   __shared__ double2 red[kThreads * V];
   __shared__ double2 channels[kSharedChannels];
@@ -286,6 +288,9 @@ __global__ void __launch_bounds__(kThreads, 2) norm_samples_kernel(const NormArg
   __syncthreads();
   const unsigned epoch = epoch_s;
   for (unsigned item = item_s; item < 2 * units; item = item_s) {
+    // The next item is asked for now; it is read behind this one's end.
+    unsigned next = 0;
+    if (threadIdx.x == 0) next = atomicAdd(p.words, 1u);
     const unsigned turn = item - lead;  // used from item `lead` on
     bool sums;
     unsigned unit;
@@ -316,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_samples_kernel(const NormArg
       apply_item<T, V, ACT, BWD>(p, unit, tx, ty);
     }
     __syncthreads();
-    if (threadIdx.x == 0) item_s = atomicAdd(p.words, 1u);
+    if (threadIdx.x == 0) item_s = next;
     __syncthreads();
   }
   if (threadIdx.x == 0) finish_words(p.words, epoch, gridDim.x);
@@ -594,9 +599,10 @@ int launch(Device* d, NormArgs<T> p) {
   const int tx = (int)(lanes < kThreads ? lanes : kThreads), ty = kThreads / tx;
   const void* kernel = (const void*)norm_samples_kernel<T, V, ACT, BWD>;
   const int64_t wave = resident_blocks(d, kernel, kThreads);
-  // About four items per block and pass, each at least four positions per thread.
-  int64_t chunks = ceil_div(wave * 4, p.N);
+  int64_t chunks = ceil_div(wave * PB_ITEMS, p.N);
   const int64_t most = ceil_div(p.S, (int64_t)ty * 4);
+  const int64_t least = ceil_div(p.S, (int64_t)ty * PB_ROWS);
+  if (chunks < least) chunks = least;
   if (chunks > most) chunks = most;
   p.rows = ceil_div(p.S, chunks);
   p.chunks = ceil_div(p.S, p.rows);
@@ -620,7 +626,7 @@ int launch(Device* d, NormArgs<T> p) {
   PB_CHECK(epoch_words(d, kFlagWords + (size_t)p.N, &p.words));
   p.err = d->err_dev;
   const int64_t grid = 2 * units < wave ? 2 * units : wave;
-  const int64_t lead = p.chunks + grid < units ? p.chunks + grid : units;
+  const int64_t lead = p.chunks + 2 * grid < units ? p.chunks + 2 * grid : units;
   PB_CHECK(kt_begin(d));
   norm_samples_kernel<T, V, ACT, BWD>
       <<<(unsigned)grid, kThreads, 0, d->stream>>>(p, tx, ty, (unsigned)units, (unsigned)lead);

@@ -43,21 +43,48 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& r) {
 
 __device__ __forceinline__ float exp_of(float x) { return expf(x); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
-__device__ __forceinline__ float reciprocal(float x) { return __fdividef(1.0f, x); }
-__device__ __forceinline__ double reciprocal(double x) { return 1.0 / x; }
+
+// 2^x and 1/x of the special-function unit: within 2 ulp and 1 ulp, results and
+// operands below 2^-126 as zero.
+__device__ __forceinline__ float exp2_unit(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_unit(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
 // s = 1 / (1 + e^-z) and rest = 1 - s, each to a few roundings of its own size:
 // with e = e^-|z| <= 1 the two are 1/(1+e) and e/(1+e), so neither is the
-// difference of two nearly equal numbers.  1 + e lies in [1, 2], where the
-// fast float32 division is within 2 ulp.
-template <typename T>
-__device__ __forceinline__ void sigmoid_pair(T z, T* s, T* rest) {
-  const T e = exp_of(z < T(0) ? z : -z);
-  const T big = reciprocal(T(1) + e), small = e * big;
-  const bool neg = z < T(0);
-  *s = neg ? small : big;
-  *rest = neg ? big : small;
+// difference of two nearly equal numbers.
+__device__ __forceinline__ void sigmoid_pair(float z, float* s, float* rest) {
+  // e = 2^(t + r) with t = -|z| log2 e rounded and r what the rounding lost (log2 e
+  // in two parts): 2^t (1 + r ln 2), r being below 2^-17.  From |z| = 126 on, e is
+  // zero; the minimum keeps a NaN.
+  constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596303e-8f, kLn2 = 0.693147182f;
+  float a;
+  asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(a) : "f"(fabsf(z)));
+  const float t = a * -kLog2e;
+  const float r = fmaf(-a, kLog2eLow, fmaf(-a, kLog2e, -t));
+  float e = exp2_unit(t);
+  e = fmaf(e, r * kLn2, e);
+  const float big = reciprocal_unit(1.0f + e), small = e * big;
+  *s = z < 0.0f ? small : big;
+  *rest = z < 0.0f ? big : small;
 }
+__device__ __forceinline__ void sigmoid_pair(double z, double* s, double* rest) {
+  const double e = exp(-fabs(z)), big = 1.0 / (1.0 + e), small = e * big;
+  *s = z < 0.0 ? small : big;
+  *rest = z < 0.0 ? big : small;
+}
+
+// s alone, where an error of |z| roundings does no harm: an activation's
+// result z s is off by that much of itself, below a rounding of z where s is small.
+__device__ __forceinline__ float sigmoid(float z) { return reciprocal_unit(1.0f + exp2_unit(z * -1.44269502f)); }
+__device__ __forceinline__ double sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
 
 // ---- flags between the blocks of one launch (words of epoch_words()) ----
 //
