@@ -35,7 +35,7 @@ struct NormArgs {
   T* out;             // y or dx
   T *mean, *rstd;     // forward: outputs, may be null; backward: inputs
   T *dweight, *dbias; // may be null
-  double2* chan;      // per-channel sums of each (n, chunk): backward, and forward beyond kSharedChannels
+  double2* chan;      // per-channel sums: of each (n, chunk), or of each block of the ring
   double2* part;      // (N, chunks, G): per-group sums
   double2* group;     // (N, G): forward (mean, rstd); backward (mean of w dz, mean of w dz xhat)
   unsigned* words;    // see pb_layers.cuh: a flag per sample
@@ -87,6 +87,174 @@ __device__ __forceinline__ double shift_of(const NormArgs<T>& p, int64_t n, int6
 // Channels whose sums a block holds in shared memory.
 constexpr int64_t kSharedChannels = 1024;
 
+// What a thread needs of its V channels: the sums of one pass over positions.
+// Backward, xhat = rstd d with d = x - mean, so the second sum is formed of
+// dz d and takes its factor rstd at the end.  Two positions at a time: their
+// terms are added in T and the pair in float64, which halves the conversions (they
+// share a unit of a sixteenth of the rate with the exponential) for one rounding more.
+template <typename T, int V, int ACT, bool BWD>
+struct ChannelSums {
+  double s1[V], s2[V];
+  double k[BWD ? 1 : V];
+  T mean[BWD ? V : 1], rstd[BWD ? V : 1], rw[BWD ? V : 1], b[BWD ? V : 1];
+
+  __device__ __forceinline__ void begin(const NormArgs<T>& p, int64_t n, int64_t c, bool on) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      s1[i] = s2[i] = 0.0;
+      const int64_t g = on ? fdiv(c + i, p.by_m) : 0;
+      if constexpr (BWD) {
+        mean[i] = __ldg(p.mean + n * p.G + g);
+        rstd[i] = __ldg(p.rstd + n * p.G + g);
+        rw[i] = on && p.weight ? rstd[i] * __ldg(p.weight + c + i) : rstd[i];
+        b[i] = on && p.bias ? __ldg(p.bias + c + i) : T(0);
+      } else {
+        k[i] = shift_of(p, n, g);
+      }
+    }
+  }
+  __device__ __forceinline__ void term(int i, T x, T dy, T* dz, T* product) const {
+    const T d = x - mean[i];
+    *dz = dy * slope<T, ACT>(fma(d, rw[i], b[i]));
+    *product = *dz * d;
+  }
+  __device__ __forceinline__ void add(const Pack<T, V>& x, const Pack<T, V>& dy) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if constexpr (BWD) {
+        T dz, product;
+        term(i, x.v[i], dy.v[i], &dz, &product);
+        s1[i] += (double)dz;
+        s2[i] += (double)product;
+      } else {
+        const double v = (double)x.v[i] - k[i];
+        s1[i] += v;
+        s2[i] = fma(v, v, s2[i]);
+      }
+    }
+  }
+  __device__ __forceinline__ void add2(const Pack<T, V>& x0, const Pack<T, V>& dy0, const Pack<T, V>& x1,
+                                       const Pack<T, V>& dy1) {
+    if constexpr (BWD) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        T z0, z1, q0, q1;
+        term(i, x0.v[i], dy0.v[i], &z0, &q0);
+        term(i, x1.v[i], dy1.v[i], &z1, &q1);
+        s1[i] += (double)(z0 + z1);
+        s2[i] += (double)(q0 + q1);
+      }
+    } else {
+      add(x0, dy0);
+      add(x1, dy1);
+    }
+  }
+  __device__ __forceinline__ void end() {
+    if constexpr (BWD) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) s2[i] *= (double)rstd[i];
+    }
+  }
+};
+
+// ... and its results, y = act(d rw + b) with rw = rstd w, and
+// dx = rstd (w dz - m1 - xhat m2) = rw dz - rstd m1 - d rstd^2 m2.
+template <typename T, int V, int ACT, bool BWD>
+struct ChannelResults {
+  T mean[V], rw[V], b[V];
+  T r1[V];                 // backward: -rstd m1; forward: the mean's low part, so that its rounding does not show
+  T r2[BWD ? V : 1];       // -rstd^2 m2
+
+  // The statistics of sample n, at `stats` or in p.group.
+  __device__ __forceinline__ void begin(const NormArgs<T>& p, int64_t n, int64_t c, bool on, const double2* stats) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int64_t g = on ? fdiv(c + i, p.by_m) : 0;
+      const double2 t = stats ? stats[g] : __ldcg(p.group + n * p.G + g);
+      const T w = on && p.weight ? __ldg(p.weight + c + i) : T(1);
+      b[i] = on && p.bias ? __ldg(p.bias + c + i) : T(0);
+      if constexpr (BWD) {
+        mean[i] = __ldg(p.mean + n * p.G + g);
+        const double r = (double)__ldg(p.rstd + n * p.G + g);
+        rw[i] = (T)(r * (double)w);
+        r1[i] = (T)(-r * t.x);
+        r2[i] = (T)(-r * r * t.y);
+      } else {
+        mean[i] = (T)t.x;
+        r1[i] = (T)(t.x - (double)mean[i]);
+        rw[i] = (T)(t.y * (double)w);
+      }
+    }
+  }
+  __device__ __forceinline__ Pack<T, V> of(const Pack<T, V>& x, const Pack<T, V>& dy) const {
+    Pack<T, V> o;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      T d = x.v[i] - mean[i];
+      if constexpr (BWD) {
+        const T dz = dy.v[i] * slope<T, ACT>(fma(d, rw[i], b[i]));
+        o.v[i] = fma(rw[i], dz, fma(d, r2[i], r1[i]));
+      } else {
+        d -= r1[i];
+        o.v[i] = activate<T, ACT>(fma(d, rw[i], b[i]));
+      }
+    }
+    return o;
+  }
+};
+
+// The first kThreads threads of a block: all of them, or those besides a
+// warp that copies.
+template <bool ALL>
+__device__ __forceinline__ void sync_threads() {
+  if constexpr (ALL) __syncthreads();
+  else asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+}
+
+// Over the ty rows of threads, in row order: the sums of tx * V channels from c0
+// on, to `out` and to `copy`, which with `more` holds earlier ones that they join.
+template <typename T, int V, bool ALL, typename S>
+__device__ __forceinline__ void sum_rows(const NormArgs<T>& p, const S& sums, int64_t c0, int tx, int ty, double2* red,
+                                         double2* out, double2* copy, bool more = false) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    red[threadIdx.x] = make_double2(sums.s1[i], sums.s2[i]);
+    sync_threads<ALL>();
+    const int64_t c = c0 + (int64_t)threadIdx.x * V + i;
+    if ((int)threadIdx.x < tx && c < p.C) {
+      double2 t = red[threadIdx.x];
+      for (int y = 1; y < ty; ++y) {
+        t.x += red[y * tx + threadIdx.x].x;
+        t.y += red[y * tx + threadIdx.x].y;
+      }
+      out[c] = t;
+      if (copy && copy != out) {
+        if (more) {
+          t.x += copy[c].x;
+          t.y += copy[c].y;
+        }
+        copy[c] = t;
+      }
+    }
+    sync_threads<ALL>();
+  }
+}
+
+// Over the channels of each group.
+template <typename T, bool BWD>
+__device__ __forceinline__ void sum_groups(const NormArgs<T>& p, const double2* channels, double2* part) {
+  for (int64_t g = threadIdx.x; g < p.G; g += kThreads) {
+    double2 t = make_double2(0.0, 0.0);
+    for (int64_t c = g * p.m; c < (g + 1) * p.m; ++c) {
+      const double2 v = channels[c];
+      const double w = BWD && p.weight ? (double)__ldg(p.weight + c) : 1.0;
+      t.x = fma(w, v.x, t.x);
+      t.y = fma(w, v.y, t.y);
+    }
+    part[g] = t;
+  }
+}
+
 // The group sums of one item: threads form tx lanes over packs of V channels
 // and ty rows.
 template <typename T, int V, int ACT, bool BWD>
@@ -98,113 +266,68 @@ __device__ __forceinline__ void sums_item(const NormArgs<T>& p, int64_t unit, in
   for (int64_t c0 = 0; c0 < p.C; c0 += (int64_t)tx * V) {
     const int64_t c = c0 + (int64_t)lx * V;
     const bool on = ly < ty && c < p.C;
-    double s1[V] = {}, s2[V] = {};
+    ChannelSums<T, V, ACT, BWD> sums;
+    sums.begin(p, n, c, on);
     if (on) {
-      double k[V];
-      T mean[V], rstd[V], w[V], b[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int64_t g = fdiv(c + i, p.by_m);
-        if constexpr (BWD) {
-          mean[i] = __ldg(p.mean + n * p.G + g);
-          rstd[i] = __ldg(p.rstd + n * p.G + g);
-          w[i] = p.weight ? __ldg(p.weight + c + i) : T(1);
-          b[i] = p.bias ? __ldg(p.bias + c + i) : T(0);
-        } else {
-          k[i] = shift_of(p, n, g);
-        }
-      }
-      const T* x = p.x + (n * p.S + r0 + ly) * p.C + c;
-      const T* dy = BWD ? p.dy + (n * p.S + r0 + ly) * p.C + c : nullptr;
+      int64_t at = (n * p.S + r0 + ly) * p.C + c;
 #pragma unroll 4
-      for (int64_t r = r0 + ly; r < r1; r += ty) {
-        const Pack<T, V> q = load_pack<T, V>(x);
-        x += ty * p.C;
-        if constexpr (BWD) {
-          const Pack<T, V> e = load_pack<T, V>(dy);
-          dy += ty * p.C;
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const T xh = (q.v[i] - mean[i]) * rstd[i];
-            const T dz = e.v[i] * slope<T, ACT>(fma(xh, w[i], b[i]));
-            s1[i] += (double)dz;
-            s2[i] += (double)(dz * xh);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const double v = (double)q.v[i] - k[i];
-            s1[i] += v;
-            s2[i] = fma(v, v, s2[i]);
-          }
-        }
+      for (int64_t r = r0 + ly; r < r1; r += ty, at += ty * p.C) {
+        const Pack<T, V> x = load_pack<T, V>(p.x + at);
+        Pack<T, V> dy;
+        if constexpr (BWD) dy = load_pack<T, V>(p.dy + at);
+        sums.add(x, dy);
       }
     }
-    // Over the rows of threads, in row order.
-#pragma unroll
-    for (int i = 0; i < V; ++i) red[i * kThreads + threadIdx.x] = make_double2(s1[i], s2[i]);
-    __syncthreads();
-    for (int q = threadIdx.x; q < tx * V; q += kThreads) {
-      const int i = q % V, l = q / V;
-      if (c0 + q >= p.C) break;
-      double2 t = red[i * kThreads + l];
-      for (int y = 1; y < ty; ++y) {
-        t.x += red[i * kThreads + y * tx + l].x;
-        t.y += red[i * kThreads + y * tx + l].y;
-      }
-      out[c0 + q] = t;
-      if (BWD && out == shared && p.chan) p.chan[unit * p.C + c0 + q] = t;
-    }
-    __syncthreads();
+    sums.end();
+    sum_rows<T, V, true>(p, sums, c0, tx, ty, red, out, BWD && p.chan ? p.chan + unit * p.C : nullptr);
   }
-  // Over the channels of each group.
-  for (int64_t g = threadIdx.x; g < p.G; g += kThreads) {
-    double2 t = make_double2(0.0, 0.0);
-    for (int64_t c = g * p.m; c < (g + 1) * p.m; ++c) {
-      const double2 v = out[c];
-      const double w = BWD && p.weight ? (double)__ldg(p.weight + c) : 1.0;
-      t.x = fma(w, v.x, t.x);
-      t.y = fma(w, v.y, t.y);
-    }
-    p.part[unit * p.G + g] = t;
+  sum_groups<T, BWD>(p, out, p.part + unit * p.G);
+}
+
+// Mean and rstd (forward) or the two means (backward) of a group from its sums.
+template <typename T, bool BWD>
+__device__ __forceinline__ double2 statistics(const NormArgs<T>& p, int64_t n, int64_t g, double2 t) {
+  const double count = (double)p.S * (double)p.m;
+  t.x /= count;
+  t.y /= count;
+  if constexpr (!BWD) {
+    // A set with NaN or Inf in it has a NaN variance (fmax alone would drop
+    // it); finite float64 values whose squares overflow have an infinite one.
+    const double var = isinf(t.y) ? t.y : fmax(fma(-t.x, t.x, t.y), 0.0);
+    const double rstd = isfinite(t.x) ? 1.0 / sqrt(var + p.eps) : t.x - t.x;
+    t = make_double2(t.x + shift_of(p, n, g), rstd);
   }
+  return t;
 }
 
 // The statistics of a sample from its items' group sums.  The threads take
 // (group, every lanes-th item) and meet in shared memory.
-template <typename T, bool BWD>
+template <typename T, bool BWD, bool ALL>
 __device__ __forceinline__ void merge_sample(const NormArgs<T>& p, int64_t n, double2* red) {
   const int wide = p.G < kThreads ? (int)p.G : kThreads, lanes = kThreads / wide;
   const int lg = threadIdx.x % wide, lk = threadIdx.x / wide;
-  const double count = (double)p.S * (double)p.m;
   for (int64_t g0 = 0; g0 < p.G; g0 += wide) {
     const int64_t g = g0 + lg;
     double2 t = make_double2(0.0, 0.0);
     if (g < p.G && lk < lanes) {
       const double2* q = p.part + (n * p.chunks + lk) * p.G + g;
-#pragma unroll 4
+#pragma unroll 16
       for (int64_t k = lk; k < p.chunks; k += lanes, q += (int64_t)lanes * p.G) {
         const double2 v = __ldcg(q);
         t.x += v.x;
         t.y += v.y;
       }
     }
-    __syncthreads();
+    sync_threads<ALL>();
     red[threadIdx.x] = t;
-    __syncthreads();
+    sync_threads<ALL>();
     if (lk == 0 && g < p.G) {
       for (int k = 1; k < lanes; ++k) {
         t.x += red[k * wide + lg].x;
         t.y += red[k * wide + lg].y;
       }
-      t.x /= count;
-      t.y /= count;
+      t = statistics<T, BWD>(p, n, g, t);
       if constexpr (!BWD) {
-        // A set with NaN or Inf in it has a NaN variance (fmax alone would drop
-        // it); finite float64 values whose squares overflow have an infinite one.
-        const double var = isinf(t.y) ? t.y : fmax(fma(-t.x, t.x, t.y), 0.0);
-        const double rstd = isfinite(t.x) ? 1.0 / sqrt(var + p.eps) : t.x - t.x;
-        t = make_double2(t.x + shift_of(p, n, g), rstd);
         if (p.mean) p.mean[n * p.G + g] = (T)t.x;
         if (p.rstd) p.rstd[n * p.G + g] = (T)t.y;
       }
@@ -219,47 +342,15 @@ __device__ __forceinline__ void apply_item(const NormArgs<T>& p, int64_t unit, i
   const int64_t n = fdiv(unit, p.by_chunks), chunk = unit - n * p.chunks;
   const int64_t r0 = chunk * p.rows, r1 = min(p.S, r0 + p.rows);
   for (int64_t c = (int64_t)lx * V; c < p.C && ly < ty; c += (int64_t)tx * V) {
-    T mean[V], low[V], rstd[V], w[V], b[V], m1[V], m2[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int64_t g = fdiv(c + i, p.by_m);
-      const double2 t = __ldcg(p.group + n * p.G + g);
-      w[i] = p.weight ? __ldg(p.weight + c + i) : T(1);
-      b[i] = p.bias ? __ldg(p.bias + c + i) : T(0);
-      if constexpr (BWD) {
-        mean[i] = __ldg(p.mean + n * p.G + g);
-        rstd[i] = __ldg(p.rstd + n * p.G + g);
-        m1[i] = (T)t.x;
-        m2[i] = (T)t.y;
-      } else {
-        // The mean in two parts, so that its rounding does not show where
-        // the values lie far from zero.
-        mean[i] = (T)t.x;
-        low[i] = (T)(t.x - (double)mean[i]);
-        rstd[i] = (T)t.y;
-      }
-    }
+    ChannelResults<T, V, ACT, BWD> results;
+    results.begin(p, n, c, true, nullptr);
     int64_t at = (n * p.S + r0 + ly) * p.C + c;
 #pragma unroll 4
     for (int64_t r = r0 + ly; r < r1; r += ty, at += ty * p.C) {
-      const Pack<T, V> q = load_pack<T, V>(p.x + at);
-      Pack<T, V> o;
-      if constexpr (BWD) {
-        const Pack<T, V> e = load_pack<T, V>(p.dy + at);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const T xh = (q.v[i] - mean[i]) * rstd[i];
-          const T dz = e.v[i] * slope<T, ACT>(fma(xh, w[i], b[i]));
-          o.v[i] = rstd[i] * (fma(w[i], dz, -m1[i]) - xh * m2[i]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const T xh = ((q.v[i] - mean[i]) - low[i]) * rstd[i];
-          o.v[i] = activate<T, ACT>(fma(xh, w[i], b[i]));
-        }
-      }
-      store_pack<T, V>(p.out + at, o);
+      const Pack<T, V> x = load_pack<T, V>(p.x + at);
+      Pack<T, V> dy;
+      if constexpr (BWD) dy = load_pack<T, V>(p.dy + at);
+      store_pack<T, V>(p.out + at, results.of(x, dy));
     }
   }
 }
@@ -268,16 +359,10 @@ __device__ __forceinline__ void apply_item(const NormArgs<T>& p, int64_t unit, i
 // turn, then the rest of apply.  lead is a sample's items and two per block (the
 // one it works on and the one it holds), so apply item j comes behind all sums of its
 // sample.
-#ifndef PB_ITEMS
-#define PB_ITEMS 2
-#define PB_ROWS 64
-#define PB_FB 3
-#define PB_BB 2
-#endif
 template <typename T, int V, int ACT, bool BWD>
-__global__ void __launch_bounds__(kThreads, BWD ? PB_BB : PB_FB) norm_samples_kernel(const NormArgs<T> p, int tx, int ty, unsigned units,
+__global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) norm_samples_kernel(const NormArgs<T> p, int tx, int ty, unsigned units,
                                                                    unsigned lead) {
-  __shared__ double2 red[kThreads * V];
+  __shared__ double2 red[kThreads];
   __shared__ double2 channels[kSharedChannels];
   __shared__ unsigned item_s, epoch_s;
   __shared__ bool last;
@@ -307,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, BWD ? PB_BB : PB_FB) norm_samples_ke
       __syncthreads();
       if (last) {
         __threadfence();
-        merge_sample<T, BWD>(p, n, red);
+        merge_sample<T, BWD, true>(p, n, red);
         __threadfence();
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -325,6 +410,292 @@ __global__ void __launch_bounds__(kThreads, BWD ? PB_BB : PB_FB) norm_samples_ke
     __syncthreads();
   }
   if (threadIdx.x == 0) finish_words(p.words, epoch, gridDim.x);
+}
+
+// ---- the same, fed by bulk copies ----------------------------------------
+//
+// Positions of a sample are one run of memory, so where rows are whole 16-byte
+// pieces one thread of each block copies them into a ring of shared-memory stages,
+// ahead of the block across the ends of runs and passes.  There is one block per SM,
+// all resident (a cooperative launch).  They work on `together` samples at a
+// time, `chunks` blocks for each: a block forms the sums of its run of positions,
+// waits until all blocks of the sample have theirs, adds them up and applies the
+// statistics to the same run, of which the last stages are still in shared memory
+// and the others come from L2.  What is left besides the copies is the chain
+// between the passes (sums over the block's rows and groups, publishing,
+// waiting, adding up), about 5 us for each round of samples.
+constexpr int kRingThreads = 480;  // and a warp that copies: 16 warps, 128 registers each thread
+constexpr int kRingWarps = kRingThreads / 32;
+constexpr int kRing = 8;
+constexpr size_t kRingSmem = 220 * 1024;
+// Up to so many (block, group) sums of a sample every block adds up for itself;
+// beyond, each block does some of the groups and all meet once more.
+constexpr int64_t kOwnSums = 8192, kOwnGroups = 512;
+
+__device__ __forceinline__ void ring_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kRingThreads) : "memory");
+}
+
+// Wait (the whole block) until `count` blocks have arrived at *counter.
+__device__ __forceinline__ void arrive_and_wait(unsigned* counter, unsigned count, int* err) {
+  __threadfence();
+  ring_sync();
+  if (threadIdx.x == 0) {
+    atomicAdd(counter, 1u);
+    if (load_acquire(counter) < count) {
+      unsigned long long t0, t;
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+      while (load_acquire(counter) < count) {
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+        if (t - t0 > kFlagWaitNs) {
+          atomicExch(err, KERR_WAIT_TIMEOUT);
+          break;
+        }
+      }
+    }
+  }
+  ring_sync();
+}
+
+template <typename T, int V, int ACT, bool BWD>
+__global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const NormArgs<T> p, int tx, int ty,
+                                                                       int stage_rows, int64_t together) {
+  constexpr int kArrays = BWD ? 2 : 1;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) uint64_t full[kRing], empty[kRing];
+  __shared__ int failed;
+  __shared__ bool last;
+  const int C = (int)p.C, G = (int)p.G, m = (int)p.m, array = stage_rows * C;  // values of one array of a stage
+  T* const ring = reinterpret_cast<T*>(smem);
+  double2* const red = reinterpret_cast<double2*>(ring + (size_t)kRing * kArrays * array);  // [V * kRingThreads]
+  double2* const channels = red + V * kRingThreads;                                          // [C]
+  double2* const stats = channels + C;  // [G] where a block adds up for itself
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kRing; ++s) {
+      barrier_init(full + s, 1);
+      barrier_init(empty + s, kRingWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    failed = 0;
+  }
+  __syncthreads();
+  const int64_t place = blockIdx.x / p.chunks, chunk = blockIdx.x - place * p.chunks;
+  const int64_t r0 = chunk * p.rows, r1 = min(p.S, r0 + p.rows);
+  const int stages = (int)((r1 - r0 + stage_rows - 1) / stage_rows);
+  // The sums leave the last `held` stages where they are; the second pass takes
+  // those first and then the others, in order.
+  const int held = min(stages, kRing);
+  unsigned turn = 0;  // copies so far: stage turn % kRing, its use number turn / kRing
+
+  if (threadIdx.x >= kRingThreads) {
+    if (threadIdx.x > kRingThreads) return;
+    bool ok = true;
+    for (int64_t n = place; n < p.N && ok; n += together) {
+      for (int k = 0; k < 2 * stages - held && ok; ++k, ++turn) {
+        const int s = turn % kRing;
+        if (turn >= kRing) ok = barrier_wait(empty + s, (turn / kRing - 1) & 1, &failed, p.err);
+        if (!ok) break;
+        const int64_t r = r0 + (int64_t)(k < stages ? k : k - stages) * stage_rows;
+        const int rows = (int)min((int64_t)stage_rows, r1 - r);
+        const unsigned bytes = (unsigned)(rows * C) * (unsigned)sizeof(T);
+        const int64_t at = (n * p.S + r) * p.C;
+        T* const to = ring + (size_t)s * kArrays * array;
+        barrier_expect(full + s, bytes * kArrays);
+        bulk_copy(to, p.x + at, bytes, full + s);
+        if constexpr (BWD) bulk_copy(to + array, p.dy + at, bytes, full + s);
+      }
+    }
+    // Nothing may be on its way when the block ends.
+    for (unsigned q = turn > kRing ? turn - kRing : 0; q < turn; ++q)
+      barrier_wait(full + q % kRing, (q / kRing) & 1, &failed, p.err);
+    return;
+  }
+
+  const int lx = threadIdx.x % tx, ly = threadIdx.x / tx;
+  const int c = lx * V;
+  const bool on = ly < ty;
+  // Stage k of the run, as copied in turn t: `two` takes two of its positions,
+  // `one` the last of an odd number.
+  auto take = [&](unsigned t, int k, int64_t n, bool wait, bool release, auto&& two, auto&& one) {
+    const int s = t % kRing;
+    if (wait) barrier_wait(full + s, (t / kRing) & 1, &failed, p.err);
+    const T* const from = ring + (size_t)s * kArrays * array + c;
+    const int64_t r = r0 + (int64_t)k * stage_rows;
+    const int rows = on ? (int)min((int64_t)stage_rows, r1 - r) : 0;
+    const int64_t at = (n * p.S + r) * p.C + c;
+    int q = ly;
+    for (; q + ty < rows; q += 2 * ty) {
+      const T* const f0 = from + q * C;
+      const T* const f1 = f0 + ty * C;
+      const Pack<T, V> x0 = *reinterpret_cast<const Pack<T, V>*>(f0), x1 = *reinterpret_cast<const Pack<T, V>*>(f1);
+      Pack<T, V> d0, d1;
+      if constexpr (BWD) {
+        d0 = *reinterpret_cast<const Pack<T, V>*>(f0 + array);
+        d1 = *reinterpret_cast<const Pack<T, V>*>(f1 + array);
+      }
+      two(x0, d0, x1, d1, at + q * C, at + (q + ty) * C);
+    }
+    if (q < rows) {
+      const T* const f0 = from + q * C;
+      const Pack<T, V> x0 = *reinterpret_cast<const Pack<T, V>*>(f0);
+      Pack<T, V> d0;
+      if constexpr (BWD) d0 = *reinterpret_cast<const Pack<T, V>*>(f0 + array);
+      one(x0, d0, at + q * C);
+    }
+    if (release) {
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) barrier_arrive(empty + s);
+    }
+  };
+  using P = const Pack<T, V>&;
+  const bool own = p.chunks * G <= kOwnSums && G <= kOwnGroups;
+  const int lanes = tx * V;                                          // channels that the threads cover, C or a little more
+  const int parts = lanes < kRingThreads ? kRingThreads / lanes : 1;  // threads per channel in the sums over rows
+  for (int64_t n = place; n < p.N; n += together) {
+    const int64_t unit = n * p.chunks + chunk;
+    {
+      ChannelSums<T, V, ACT, BWD> sums;
+      sums.begin(p, n, c, on);
+      for (int k = 0; k < stages; ++k)
+        take(turn + k, k, n, true, k < stages - held,
+             [&](P x0, P d0, P x1, P d1, int64_t, int64_t) { sums.add2(x0, d0, x1, d1); },
+             [&](P x, P dy, int64_t) { sums.add(x, dy); });
+      sums.end();
+      // Over the rows of threads: red is [ty][tx * V], `parts` threads per channel.
+      if (on) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) red[(ly * V + i) * tx + lx] = make_double2(sums.s1[i], sums.s2[i]);
+      }
+    }
+    ring_sync();
+    if ((int)threadIdx.x < parts * lanes) {
+      const int q = threadIdx.x % lanes, part = threadIdx.x / lanes;
+      double2 t = make_double2(0.0, 0.0);
+      for (int y = part; y < ty; y += parts) {
+        const double2 v = red[y * lanes + q];
+        t.x += v.x;
+        t.y += v.y;
+      }
+      if (part < ty) red[part * lanes + q] = t;
+    }
+    for (int q = threadIdx.x + kRingThreads; q < lanes; q += kRingThreads) {  // more channels than threads: parts is 1
+      for (int y = 1; y < ty; ++y) {
+        red[q].x += red[y * lanes + q].x;
+        red[q].y += red[y * lanes + q].y;
+      }
+    }
+    ring_sync();
+    for (int q = threadIdx.x; q < lanes; q += kRingThreads) {
+      double2 t = red[q];
+      for (int k = 1; k < parts && k < ty; ++k) {
+        t.x += red[k * lanes + q].x;
+        t.y += red[k * lanes + q].y;
+      }
+      const int ch = q % tx * V + q / tx;
+      if (ch < C) {
+        if (BWD && p.chan) {
+          double2* const all = p.chan + (int64_t)blockIdx.x * C + ch;  // over the block's samples
+          const double2 before = n == place ? make_double2(0.0, 0.0) : *all;
+          *all = make_double2(before.x + t.x, before.y + t.y);
+        }
+        if (BWD && p.weight) {
+          const double w = (double)__ldg(p.weight + ch);
+          t.x *= w;
+          t.y *= w;
+        }
+        channels[ch] = t;
+      }
+    }
+    ring_sync();
+    // Over the channels of each group: a thread each, or a warp where they are many.
+    if (m <= 16) {
+      for (int g = threadIdx.x; g < G; g += kRingThreads) {
+        double2 t = channels[g * m];
+        for (int k = 1; k < m; ++k) {
+          t.x += channels[g * m + k].x;
+          t.y += channels[g * m + k].y;
+        }
+        __stcg(p.part + unit * G + g, t);
+      }
+    } else {
+      for (int g = threadIdx.x / 32; g < G; g += kRingWarps) {
+        double2 t = make_double2(0.0, 0.0);
+        for (int k = threadIdx.x & 31; k < m; k += 32) {
+          t.x += channels[g * m + k].x;
+          t.y += channels[g * m + k].y;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
+          t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
+        }
+        if ((threadIdx.x & 31) == 0) __stcg(p.part + unit * G + g, t);
+      }
+    }
+    // Over the blocks of the sample.
+    if (p.chunks > 1) arrive_and_wait(p.arrivals + n, (unsigned)p.chunks, p.err);
+    else ring_sync();
+    const int wide = min(G, kRingThreads), rows = kRingThreads / wide;
+    const int first = own ? 0 : (int)chunk, step = own ? 1 : (int)p.chunks;  // groups this block adds up
+    for (int g0 = 0; g0 * step + first < G; g0 += wide) {
+      const int g = (g0 + (int)threadIdx.x % wide) * step + first, row = threadIdx.x / wide;
+      double2 t = make_double2(0.0, 0.0);
+      if (g < G && row < rows) {
+        const double2* q = p.part + (n * p.chunks + row) * G + g;
+#pragma unroll 8
+        for (int64_t k = row; k < p.chunks; k += rows, q += (int64_t)rows * G) {
+          const double2 v = __ldcg(q);
+          t.x += v.x;
+          t.y += v.y;
+        }
+      }
+      red[threadIdx.x] = t;
+      ring_sync();
+      if (row == 0 && g < G) {
+        for (int k = 1; k < rows; ++k) {
+          t.x += red[k * wide + threadIdx.x].x;
+          t.y += red[k * wide + threadIdx.x].y;
+        }
+        t = statistics<T, BWD>(p, n, g, t);
+        if (own) stats[g] = t;
+        else __stcg(p.group + n * G + g, t);
+        if (!BWD && (!own || chunk == 0)) {
+          if (p.mean) p.mean[n * G + g] = (T)t.x;
+          if (p.rstd) p.rstd[n * G + g] = (T)t.y;
+        }
+      }
+      ring_sync();
+    }
+    if (!own) {
+      if (p.chunks > 1) arrive_and_wait(p.arrivals + n, 2 * (unsigned)p.chunks, p.err);
+      else {
+        __threadfence();
+        ring_sync();
+      }
+    }
+    ChannelResults<T, V, ACT, BWD> results;
+    results.begin(p, n, c, on, own ? stats : nullptr);
+    auto two = [&](P x0, P d0, P x1, P d1, int64_t a0, int64_t a1) {
+      store_pack<T, V>(p.out + a0, results.of(x0, d0));
+      store_pack<T, V>(p.out + a1, results.of(x1, d1));
+    };
+    auto one = [&](P x, P dy, int64_t a) { store_pack<T, V>(p.out + a, results.of(x, dy)); };
+    for (int k = stages - held; k < stages; ++k) take(turn + k, k, n, false, true, two, one);
+    for (int k = 0; k < stages - held; ++k) take(turn + stages + k, k, n, true, true, two, one);
+    turn += 2 * stages - held;
+  }
+  // The last block to finish leaves the counters at zero.
+  if (p.chunks > 1) {
+    if (threadIdx.x == 0) {
+      __threadfence();
+      last = atomicAdd(p.words + 1, 1u) == gridDim.x - 1;
+    }
+    ring_sync();
+    if (last) {
+      for (int64_t n = threadIdx.x; n < p.N; n += kRingThreads) p.arrivals[n] = 0;
+      if (threadIdx.x == 0) p.words[1] = 0;
+    }
+  }
 }
 
 template <typename T>
@@ -509,31 +880,38 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormArgs<T> p
   }
 }
 
-// dweight and dbias: `rows` rows of per-channel sums, added in a fixed order.
+// dweight and dbias: `rows` rows of per-channel sums, added in a fixed order.  A
+// few hundred rows for each channel: 32 threads share them, since the reads'
+// latency is what this takes.
+constexpr int kAffineWarps = 32;
 template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_affine_kernel(const double2* sums, int64_t rows, int64_t C, T* dweight,
-                                                               T* dbias) {
-  __shared__ double2 red[kWarps][32];
+__global__ void __launch_bounds__(32 * kAffineWarps) norm_affine_kernel(const double2* sums, int64_t rows, int64_t C,
+                                                                        T* dweight, T* dbias) {
+  __shared__ double2 red[kAffineWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   double2 t = make_double2(0.0, 0.0);
   if (c < C) {
-#pragma unroll 4
-    for (int64_t r = warp; r < rows; r += kWarps) {
-      const double2 v = sums[r * C + c];
+#pragma unroll 8
+    for (int64_t r = warp; r < rows; r += kAffineWarps) {
+      const double2 v = __ldg(sums + r * C + c);
       t.x += v.x;
       t.y += v.y;
     }
   }
   red[warp][lane] = t;
   __syncthreads();
-  if (warp == 0 && c < C) {
-    for (int w = 1; w < kWarps; ++w) {
-      t.x += red[w][lane].x;
-      t.y += red[w][lane].y;
-    }
-    if (dbias) dbias[c] = (T)t.x;
-    if (dweight) dweight[c] = (T)t.y;
+  // Warp w adds up channel w over the lanes.
+  t = red[lane][warp];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
+    t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
+  }
+  const int64_t mine = (int64_t)blockIdx.x * 32 + warp;
+  if (lane == 0 && mine < C) {
+    if (dbias) dbias[mine] = (T)t.x;
+    if (dweight) dweight[mine] = (T)t.y;
   }
 }
 
@@ -541,7 +919,7 @@ template <typename T>
 int launch_affine(Device* d, const double2* sums, int64_t rows, const NormArgs<T>& p) {
   const int64_t blocks = ceil_div(p.C, (int64_t)32);
   if (blocks > INT32_MAX) PB_FAIL(PB_ERR_UNSUPPORTED, "too many channels");
-  norm_affine_kernel<T><<<(unsigned)blocks, kThreads, 0, d->stream>>>(sums, rows, p.C, p.dweight, p.dbias);
+  norm_affine_kernel<T><<<(unsigned)blocks, 32 * kAffineWarps, 0, d->stream>>>(sums, rows, p.C, p.dweight, p.dbias);
   PB_LAUNCHED(d);
   return PB_OK;
 }
@@ -593,27 +971,15 @@ int launch_rows_of(Device* d, int act, const NormArgs<T>& p) {
   return launch_rows<T, V, 256, 4, BWD>(d, act, p);
 }
 
-template <typename T, int V, int ACT, bool BWD>
-int launch(Device* d, NormArgs<T> p) {
-  const int64_t lanes = ceil_div(p.C, (int64_t)V);
-  const int tx = (int)(lanes < kThreads ? lanes : kThreads), ty = kThreads / tx;
-  const void* kernel = (const void*)norm_samples_kernel<T, V, ACT, BWD>;
-  const int64_t wave = resident_blocks(d, kernel, kThreads);
-  int64_t chunks = ceil_div(wave * PB_ITEMS, p.N);
-  const int64_t most = ceil_div(p.S, (int64_t)ty * 4);
-  const int64_t least = ceil_div(p.S, (int64_t)ty * PB_ROWS);
-  if (chunks < least) chunks = least;
-  if (chunks > most) chunks = most;
-  p.rows = ceil_div(p.S, chunks);
-  p.chunks = ceil_div(p.S, p.rows);
-  p.by_chunks = make_fastdiv(p.chunks);
-  p.by_m = make_fastdiv(p.m);
+// Scratch, counters and flags of the samples kernels for p.N * p.chunks units and
+// that many rows of per-channel sums.
+template <typename T, bool BWD>
+int sample_workspace(Device* d, NormArgs<T>& p, bool shared_channels, int64_t channel_sums) {
   const int64_t units = p.N * p.chunks;
   if (units >= (int64_t(1) << 30)) PB_FAIL(PB_ERR_UNSUPPORTED, "more than 2^30 samples");
-  const bool affine = BWD && (p.dweight || p.dbias);
-  const bool by_channel = affine || p.C > kSharedChannels;
+  const bool by_channel = (BWD && (p.dweight || p.dbias)) || !shared_channels;
   size_t chan = 0, part, group;
-  const int64_t e1[] = {units, p.C}, e2[] = {units, p.G}, e3[] = {p.N, p.G};
+  const int64_t e1[] = {channel_sums, p.C}, e2[] = {units, p.G}, e3[] = {p.N, p.G};
   if ((by_channel && !array_bytes(e1, 2, sizeof(double2), &chan)) || !array_bytes(e2, 2, sizeof(double2), &part) ||
       !array_bytes(e3, 2, sizeof(double2), &group))
     PB_FAIL(PB_ERR_INVALID, "extents too large");
@@ -625,6 +991,24 @@ int launch(Device* d, NormArgs<T> p) {
   if (p.chunks > 1) PB_CHECK(counters(d, (size_t)p.N, &p.arrivals));
   PB_CHECK(epoch_words(d, kFlagWords + (size_t)p.N, &p.words));
   p.err = d->err_dev;
+  p.by_chunks = make_fastdiv(p.chunks);
+  p.by_m = make_fastdiv(p.m);
+  return PB_OK;
+}
+
+template <typename T, int V, int ACT, bool BWD>
+int launch_items(Device* d, NormArgs<T> p, int tx, int ty) {
+  const void* kernel = (const void*)norm_samples_kernel<T, V, ACT, BWD>;
+  const int64_t wave = resident_blocks(d, kernel, kThreads);
+  int64_t chunks = ceil_div(wave * 2, p.N);
+  const int64_t most = ceil_div(p.S, (int64_t)ty * 4);
+  const int64_t least = ceil_div(p.S, (int64_t)ty * 64);
+  if (chunks < least) chunks = least;
+  if (chunks > most) chunks = most;
+  p.rows = ceil_div(p.S, chunks);
+  p.chunks = ceil_div(p.S, p.rows);
+  PB_CHECK((sample_workspace<T, BWD>(d, p, p.C <= kSharedChannels, p.N * p.chunks)));
+  const int64_t units = p.N * p.chunks;
   const int64_t grid = 2 * units < wave ? 2 * units : wave;
   const int64_t lead = p.chunks + 2 * grid < units ? p.chunks + 2 * grid : units;
   PB_CHECK(kt_begin(d));
@@ -632,7 +1016,55 @@ int launch(Device* d, NormArgs<T> p) {
       <<<(unsigned)grid, kThreads, 0, d->stream>>>(p, tx, ty, (unsigned)units, (unsigned)lead);
   PB_LAUNCHED(d);
   PB_CHECK(kt_end(d));
-  return affine ? launch_affine<T>(d, p.chan, units, p) : PB_OK;
+  return BWD && (p.dweight || p.dbias) ? launch_affine<T>(d, p.chan, units, p) : PB_OK;
+}
+
+template <typename T, int V, int ACT, bool BWD>
+int launch_ring(Device* d, NormArgs<T> p) {
+  constexpr int kArrays = BWD ? 2 : 1;
+  const int tx = (int)ceil_div(p.C, (int64_t)V), ty = kRingThreads / tx;
+  const int64_t row_bytes = p.C * (int64_t)sizeof(T) * kArrays;
+  const int64_t fixed = (int64_t)sizeof(double2) * (V * kRingThreads + p.C + (p.G <= kOwnGroups ? p.G : 0));
+  // The ring takes what is left of shared memory; positions per stage in
+  // pairs per thread where they fit.
+  int64_t stage_rows = ((int64_t)kRingSmem - fixed) / kRing / row_bytes;
+  if (stage_rows > 2 * ty) stage_rows = stage_rows / (2 * ty) * (2 * ty);
+  const void* kernel = (const void*)norm_ring_kernel<T, V, ACT, BWD>;
+  const size_t bytes = (size_t)(kRing * stage_rows * row_bytes + fixed);
+  PB_CHECK(allow_smem(d, kernel, kRingSmem));
+  const int64_t wave = d->sm_count;
+  // Samples worked on together: their operands stay in L2 between the passes,
+  // and a block has at least two positions per thread.
+  const int64_t most = ceil_div(p.S, (int64_t)ty * 2);
+  int64_t together = (int64_t(48) << 20) / (p.S * row_bytes);
+  if (together < ceil_div(wave, most)) together = ceil_div(wave, most);
+  if (together < 1) together = 1;
+  if (together > wave) together = wave;
+  if (together > p.N) together = p.N;
+  together = ceil_div(p.N, ceil_div(p.N, together));  // rounds of equal size
+  int64_t chunks = wave / together;
+  if (chunks > most) chunks = most;
+  p.rows = ceil_div(p.S, chunks);
+  p.chunks = ceil_div(p.S, p.rows);
+  PB_CHECK((sample_workspace<T, BWD>(d, p, true, together * p.chunks)));
+  PB_CHECK(kt_begin(d));
+  int rows = (int)stage_rows, lanes = tx, thread_rows = ty;
+  void* args[] = {&p, &lanes, &thread_rows, &rows, &together};
+  PB_CUDA(cudaLaunchCooperativeKernel(kernel, dim3((unsigned)(together * p.chunks)), dim3(kRingThreads + 32), args,
+                                      bytes, d->stream));
+  PB_LAUNCHED(d);
+  PB_CHECK(kt_end(d));
+  return BWD && (p.dweight || p.dbias) ? launch_affine<T>(d, p.chan, together * p.chunks, p) : PB_OK;
+}
+
+template <typename T, int V, int ACT, bool BWD>
+int launch(Device* d, const NormArgs<T>& p) {
+  const int64_t lanes = ceil_div(p.C, (int64_t)V);
+  const int tx = (int)(lanes < kThreads ? lanes : kThreads), ty = kThreads / tx;
+  // The ring takes rows of whole 16-byte pieces (V > 1), and at most kThreads of them.
+  if constexpr (V > 1)
+    if (lanes <= kThreads) return launch_ring<T, V, ACT, BWD>(d, p);
+  return launch_items<T, V, ACT, BWD>(d, p, tx, ty);
 }
 
 template <typename T, int V, bool BWD>

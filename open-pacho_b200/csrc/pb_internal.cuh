@@ -165,18 +165,19 @@ inline int allow_smem(Device* d, const void* kernel, size_t bytes) {
   done.insert(key);
   return PB_OK;
 }
-// Blocks of `threads` threads of `kernel` resident on d's device at once (one
-// wave), from the occupancy API, cached per (kernel, device).  Grids sized to
-// it avoid a partial second wave.
-inline int64_t resident_blocks(Device* d, const void* kernel, int threads) {
+// Blocks of `threads` threads of `kernel`, each with `dynamic_smem` bytes of
+// dynamic shared memory, resident on d's device at once (one wave), from the
+// occupancy API, cached per (kernel, device, bytes).  Grids sized to it avoid a
+// partial second wave.
+inline int64_t resident_blocks(Device* d, const void* kernel, int threads, size_t dynamic_smem = 0) {
   static std::mutex mu;
-  static std::map<std::pair<const void*, int>, int64_t> known;
+  static std::map<std::pair<std::pair<const void*, int>, size_t>, int64_t> known;
   std::lock_guard<std::mutex> g(mu);
-  const auto key = std::make_pair(kernel, d->ordinal);
+  const auto key = std::make_pair(std::make_pair(kernel, d->ordinal), dynamic_smem);
   auto it = known.find(key);
   if (it != known.end()) return it->second;
   int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0) != cudaSuccess ||
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, dynamic_smem) != cudaSuccess ||
       per_sm < 1)
     per_sm = 1;
   const int64_t n = (int64_t)per_sm * d->sm_count;

@@ -12,7 +12,7 @@ template <> struct Vec16<double> { using type = double2; static constexpr int n 
 // V values of T in registers, moved with one access when V * sizeof(T) is 16
 // (the address then has to be 16-byte aligned) and value by value otherwise.
 template <typename T, int V>
-struct Pack {
+struct alignas(V * sizeof(T) == 16 ? 16 : sizeof(T)) Pack {
   T v[V];
 };
 
@@ -128,6 +128,57 @@ __device__ __forceinline__ void finish_words(unsigned* words, unsigned epoch, un
     words[1] = 0;
     words[2] = epoch;
   }
+}
+
+// ---- runs of memory on their way into shared memory ------------------------
+//
+// Bulk copies that report to an mbarrier.  Every wait is bounded: after
+// kFlagWaitNs the error word and `failed` are set and the kernel goes on to its
+// end (with wrong values), its further waits being short.
+__device__ __forceinline__ uint32_t shared_address(const void* p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void barrier_init(uint64_t* bar, unsigned count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(bar)) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint64_t* bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool barrier_try(uint64_t* bar, unsigned parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(shared_address(bar)), "r"(parity), "r"(20000)  // sleep for up to 20 us
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool barrier_wait(uint64_t* bar, unsigned parity, volatile int* failed, int* err) {
+  if (barrier_try(bar, parity)) return true;
+  unsigned long long t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  const unsigned long long limit = *failed ? 1000 * 1000 : kFlagWaitNs;
+  while (!barrier_try(bar, parity)) {
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    if (t - t0 > limit) {
+      *failed = 1;
+      atomicExch(err, KERR_WAIT_TIMEOUT);
+      return false;
+    }
+  }
+  return true;
+}
+// `bytes` (a multiple of 16) from global to shared memory, both 16-byte aligned.
+__device__ __forceinline__ void bulk_copy(void* to, const void* from, unsigned bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(shared_address(to)),
+      "l"(from), "r"(bytes), "r"(shared_address(bar))
+      : "memory");
 }
 
 // Whether [p, p + pn) and [q, q + qn) share a byte (NULL shares none).
