@@ -6,23 +6,24 @@
 // of the chain is t = s forward and t = length - 1 - s backward.
 //
 // A column is one (outer, inner) pair; neighbouring columns are neighbours in
-// memory, so lanes run over columns and a warp's access is a row segment.
+// memory, so lanes run over columns and a warp's access is a row segment.  A lane
+// walks its chain in order, and nothing but the bytes on their way limits it: each
+// warp is a block of its own with a ring of stages in shared memory that
+// asynchronous copies fill ahead of it, so about 500 warps with 16 KiB each
+// under way keep HBM busy and no block ever waits for another.
 //
-// Many columns or few steps: a thread per column walks the chain.  Few columns
-// and many steps: the chain is cut.  n steps map x to P x + H, with P the product
-// of their coefficients and H their result from 0; both are known without the
-// value x before them, and two such maps compose to one.  A thread takes
-// L steps of a column in registers, reduces them to (P, H), and the block
-// composes its threads' maps; the block's own map goes to memory for the
-// blocks behind it, which compose the maps of the chunks before them.  With the
-// true value before its steps each thread then runs them again from registers:
-// every input is read once.
+// Fewer columns than that: the chain is cut into segments of equal length, and a
+// lane walks one segment of one column.  n steps map x to P x + H, with P the
+// product of their coefficients and H their result from 0; a first pass forms
+// the maps of the segments, and each lane of the second composes those before
+// its own to find its start.  The first pass walks each segment from its end to
+// its start (H += P u, P *= c), so that L2 holds the steps that the second
+// pass reads first.  P and H are float64: a product of thousands of gates
+// neither over- nor underflows where a float32 recurrence does not.  Every
+// composition has a fixed order, so results do not depend on timing.
 //
-// Every composition has a fixed order (chunks in groups of kGroup: the value at
-// the end of the group before, then the chunks of the own group one by one), so
-// the result does not depend on timing.  P and the composed values are float64:
-// a product of thousands of gates neither over- nor underflows where the
-// recurrence itself does not.
+// Few steps, or more columns than fill the card: a thread per column reads
+// directly (recurrence_columns_kernel).
 #include <type_traits>
 
 #include "pb_layers.cuh"
@@ -31,8 +32,8 @@ namespace pb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kGroup = 16;  // chunks per group
+constexpr int kRows = 16;        // chain steps per stage
+constexpr int kInlineMaps = 32;  // segments up to which a lane composes the maps before its own itself
 
 template <typename T>
 struct ScanArgs {
@@ -43,152 +44,128 @@ struct ScanArgs {
   T* out1;                   // backward: db
   T* last;                   // forward: final; backward: dstate; may be null
   int64_t length, inner, columns;
-  // The cut chain (recurrence_chunks_kernel).
-  int lanes_log2;            // lanes of a warp along columns
-  unsigned tiles, chunks;    // column tiles, chunks along the chain
-  double2* maps;             // [chunk][column]: (P, H)
-  double* ends;              // [group][column]: the value at a group's end
-  unsigned* words;           // ticket, finished blocks, epoch, -, then a flag per (tile, chunk) and per (tile, group)
-  int* err;
+  FastDiv by_inner, by_columns;
+  int wide;                  // 16-byte copies are aligned
+  int64_t segments, steps;   // segments of `steps` chain steps (the last may be shorter)
+  double2* maps;             // [segment][column]: (P, H)
+  double* starts;            // [segment][column]: the value before the segment (many segments)
 };
 
-__device__ __forceinline__ int64_t column_base(int64_t col, int64_t length, int64_t inner) {
-  const int64_t o = col / inner;
-  return o * length * inner + (col - o * inner);
+template <typename T>
+__device__ __forceinline__ int64_t column_base(const ScanArgs<T>& p, int64_t col) {
+  const int64_t o = fdiv(col, p.by_inner);
+  return o * p.length * p.inner + (col - o * p.inner);
 }
 
-// L consecutive chain steps of one column in registers.  Steps past the end
-// are the identity.
-template <typename T, int GATE, bool BWD, int L>
-struct Steps;
+// The value `e` elements (of the type that addresses this array) into it.  A
+// 32-bit I serves arrays below 4 GiB: one offset for all operands of a step.
+template <typename T, typename I>
+__device__ __forceinline__ const T* at(const T* p, I e) {
+  if constexpr (sizeof(I) == 4) return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + e * (I)sizeof(T));
+  else return p + e;
+}
+template <typename T, typename I>
+__device__ __forceinline__ T* at(T* p, I e) {
+  return const_cast<T*>(at(static_cast<const T*>(p), e));
+}
 
-template <typename T, int GATE, int L>
-struct Steps<T, GATE, false, L> {
-  T c[L], u[L];
+// Element of chain step s of a column.
+template <bool BWD, typename I, typename T>
+__device__ __forceinline__ I element(const ScanArgs<T>& p, I base, int64_t s) {
+  return base + (I)(BWD ? p.length - 1 - s : s) * (I)p.inner;
+}
 
-  __device__ __forceinline__ void load(const ScanArgs<T>& p, int64_t base, int64_t, int64_t s0) {
-    const int left = (int)max((int64_t)0, min((int64_t)L, p.length - s0));
-    const T* a = p.a + base + s0 * p.inner;
-    const T* b = p.b + base + s0 * p.inner;
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      c[i] = T(1);
-      u[i] = T(0);
-      if (i < left) {
-        c[i] = __ldg(a);
-        u[i] = __ldg(b);
-      }
-      a += p.inner;
-      b += p.inner;
-    }
+// One chain step.  Backward, the own gate gives the outputs and is the
+// coefficient of the next step.
+template <typename T, int GATE, bool BWD>
+struct Step;
+
+template <typename T, int GATE>
+struct Step<T, GATE, false> {
+  __device__ __forceinline__ static void operands(T a, T b, T* c, T* u) {
     if constexpr (GATE == PB_GATE_SIGMOID) {
-#pragma unroll
-      for (int i = 0; i < L; ++i) {
-        T s, rest;
-        sigmoid_pair(c[i], &s, &rest);
-        c[i] = i < left ? s : T(1);
-        u[i] *= rest;
-      }
+      T rest;
+      sigmoid_pair(a, c, &rest);
+      *u = rest * b;
+    } else {
+      *c = a;
+      *u = b;
     }
-  }
-  __device__ __forceinline__ T coefficient(int i) const { return c[i]; }
-  __device__ __forceinline__ T input(int i) const { return u[i]; }
-
-  // The outputs of these steps from the value `x` before the first of them;
-  // returns the value after the last.
-  __device__ __forceinline__ T run(const ScanArgs<T>& p, int64_t base, int64_t col, int64_t s0, T x) const {
-    const int64_t left = p.length - s0;
-    T* h = p.out0 + base + s0 * p.inner;
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      x = fma(c[i], x, u[i]);
-      if (i < left) *h = x;
-      h += p.inner;
-    }
-    if (p.last && left > 0 && left <= L) p.last[col] = x;
-    return x;
   }
 };
 
-// Backward: step i of the chain is t = t0 - i.  Its own gate gives the outputs
-// and is the coefficient of step i + 1; the first step's coefficient is the
-// gate at t0 + 1, or 1 at the end of the sequence (dfinal as it is).
-template <typename T, int GATE, int L>
-struct Steps<T, GATE, true, L> {
-  T first, alpha[L], g[L], before[L];
-  T rest[GATE == PB_GATE_SIGMOID ? L : 1], put[GATE == PB_GATE_SIGMOID ? L : 1];
-
-  __device__ __forceinline__ void load(const ScanArgs<T>& p, int64_t base, int64_t col, int64_t s0) {
-    const int left = (int)max((int64_t)0, min((int64_t)L, p.length - s0));
-    const int64_t t0 = p.length - 1 - s0;
-    int64_t e = base + t0 * p.inner;
-    first = T(1);
-    if (left > 0 && s0 > 0) first = __ldg(p.a + e + p.inner);
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      alpha[i] = T(1);
-      g[i] = before[i] = T(0);
-      if (i < left) {
-        alpha[i] = __ldg(p.a + e);
-        g[i] = __ldg(p.dh + e);
-        if (t0 > i) before[i] = __ldg(p.h + e - p.inner);
-        else if (p.state) before[i] = __ldg(p.state + col);
-        if constexpr (GATE == PB_GATE_SIGMOID) put[i] = __ldg(p.b + e);
-      }
-      e -= p.inner;
-    }
+template <typename T, int GATE>
+struct Step<T, GATE, true> {
+  __device__ __forceinline__ static T gate(T a, T* rest) {
     if constexpr (GATE == PB_GATE_SIGMOID) {
-      T unused;
-      if (s0 > 0) sigmoid_pair(first, &first, &unused);
-#pragma unroll
-      for (int i = 0; i < L; ++i) {
-        T s;
-        sigmoid_pair(alpha[i], &s, &rest[i]);
-        alpha[i] = i < left ? s : T(1);
-      }
+      T s;
+      sigmoid_pair(a, &s, rest);
+      return s;
+    } else {
+      return a;
     }
   }
-  __device__ __forceinline__ T coefficient(int i) const { return i ? alpha[i - 1] : first; }
-  __device__ __forceinline__ T input(int i) const { return g[i]; }
-
-  __device__ __forceinline__ T run(const ScanArgs<T>& p, int64_t base, int64_t col, int64_t s0, T x) const {
-    const int64_t left = p.length - s0;
-    int64_t e = base + (left - 1) * p.inner;
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      x = fma(coefficient(i), x, g[i]);
-      if (i < left) {
-        if constexpr (GATE == PB_GATE_SIGMOID) {
-          p.out1[e] = x * rest[i];
-          p.out0[e] = x * (before[i] - put[i]) * (alpha[i] * rest[i]);
-        } else {
-          p.out1[e] = x;
-          p.out0[e] = x * before[i];
-        }
-        if (p.last && left == i + 1) p.last[col] = alpha[i] * x;
-      }
-      e -= p.inner;
+  // da and db of a step with the chain value g.
+  __device__ __forceinline__ static void outputs(T g, T alpha, T rest, T before, T b, T* da, T* db) {
+    if constexpr (GATE == PB_GATE_SIGMOID) {
+      *db = g * rest;
+      *da = g * (before - b) * (alpha * rest);
+    } else {
+      *db = g;
+      *da = g * before;
     }
-    return x;
   }
 };
 
-// A thread per column, the whole chain in order.
-template <typename T, int GATE, bool BWD, int L>
+// A thread per column, the whole chain in order; the loads of kAhead steps are
+// issued together.
+template <typename T, typename I, int GATE, bool BWD>
 __global__ void __launch_bounds__(kThreads) recurrence_columns_kernel(const ScanArgs<T> p) {
+  constexpr int kAhead = 8;
   const int64_t col = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (col >= p.columns) return;
-  const int64_t base = column_base(col, p.length, p.inner);
+  const I base = (I)column_base(p, col), step = (I)p.inner;
   T x = p.start ? p.start[col] : T(0);
-  if (p.length == 0) {
-    if (p.last) p.last[col] = x;
-    return;
+  T c = T(1);  // backward: the coefficient of the next step
+  for (int64_t s0 = 0; s0 < p.length; s0 += kAhead) {
+    const int left = (int)min((int64_t)kAhead, p.length - s0);
+    I e = element<BWD>(p, base, s0);
+    T a[kAhead], b[kAhead], g[BWD ? kAhead : 1], before[BWD ? kAhead : 1];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      a[i] = b[i] = T(0);
+      if (i < left) {
+        const I q = BWD ? (I)(e - (I)i * step) : (I)(e + (I)i * step);
+        a[i] = __ldg(at(p.a, q));
+        if (!BWD || GATE == PB_GATE_SIGMOID) b[i] = __ldg(at(p.b, q));
+        if constexpr (BWD) {
+          g[i] = __ldg(at(p.dh, q));
+          if (s0 + i + 1 < p.length) before[i] = __ldg(at(p.h, (I)(q - step)));
+          else before[i] = p.state ? p.state[col] : T(0);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (i < left) {
+        const I q = BWD ? (I)(e - (I)i * step) : (I)(e + (I)i * step);
+        if constexpr (!BWD) {
+          T u;
+          Step<T, GATE, false>::operands(a[i], b[i], &c, &u);
+          x = fma(c, x, u);
+          *at(p.out0, q) = x;
+        } else {
+          x = fma(c, x, g[i]);
+          T rest = T(0), da, db;
+          c = Step<T, GATE, true>::gate(a[i], &rest);
+          Step<T, GATE, true>::outputs(x, c, rest, before[i], b[i], &da, &db);
+          *at(p.out1, q) = db;
+          *at(p.out0, q) = da;
+        }
+      }
+    }
   }
-  for (int64_t s0 = 0; s0 < p.length; s0 += L) {
-    Steps<T, GATE, BWD, L> st;
-    st.load(p, base, col, s0);
-    x = st.run(p, base, col, s0, x);
-  }
+  if (p.last) p.last[col] = BWD ? c * x : x;
 }
 
 // x -> P x + H.  0 maps to H even where P has overflowed.
@@ -200,154 +177,276 @@ __device__ __forceinline__ double2 compose(const double2& a, const double2& b) {
   return make_double2(a.x * b.x, apply(b, a.y));
 }
 
-// One block per (column tile, chunk).  A warp covers 2^lanes_log2 columns and
-// 32 >> lanes_log2 consecutive pieces of L steps, the block kWarps times that.
-// Blocks take their chunk from a counter, chunk by chunk over the column
-// tiles, so every chunk that a block waits for is already running or done.
-template <typename T, int GATE, bool BWD, int L>
-__global__ void __launch_bounds__(kThreads, BWD ? (sizeof(T) == 4 ? 3 : 2) : 4) recurrence_chunks_kernel(const ScanArgs<T> p) {
-  __shared__ double2 warp_map[kWarps][32];
-  __shared__ double2 earlier[kGroup - 1][32];
-  __shared__ double carry[32];
-  __shared__ unsigned ticket_s, epoch_s;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) {
-    ticket_s = atomicAdd(p.words, 1u);
-    epoch_s = load_acquire(p.words + 2) + 1;
-  }
-  __syncthreads();
-  const unsigned chunk = ticket_s / p.tiles, tile = ticket_s % p.tiles, epoch = epoch_s;
-  const int width = 1 << p.lanes_log2, pieces = 32 >> p.lanes_log2;
-  const int lc = lane & (width - 1), piece = lane >> p.lanes_log2;
-  const int64_t col = (int64_t)tile * width + lc;
-  const bool on = col < p.columns;
-  const int64_t base = on ? column_base(col, p.length, p.inner) : 0;
-  const int64_t s0 = (int64_t)chunk * (kWarps * L) * pieces + (int64_t)(warp * pieces + piece) * L;
-  Steps<T, GATE, BWD, L> st;
-  st.load(p, base, on ? col : 0, on ? s0 : p.length);
+// Asynchronous copy of BYTES into shared memory; zeros where `there` is false
+// (nothing is read then).
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from, bool there) {
+  const unsigned s = shared_address(to);
+  const int n = there ? BYTES : 0;
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(from), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(s), "l"(from), "n"(BYTES), "r"(n) : "memory");
+}
 
-  // This thread's map, and the composition of the pieces before it in the warp.
-  double2 map;
-  {
-    double P = (double)st.coefficient(0);
-    T H = fma(st.coefficient(0), T(0), st.input(0));
+// The operands of a stage: forward a, b; backward a, dh and, unless only maps
+// are formed, h[t - 1] and (sigmoid) b.
+template <int GATE, bool BWD, bool MAPS>
+constexpr int stream_arrays() {
+  return !BWD || MAPS ? 2 : GATE == PB_GATE_SIGMOID ? 4 : 3;
+}
+
+// A warp: lane l takes (segment, column) number blockIdx.x * 32 + l.  MAPS: the
+// first pass (from the segment's end to its start), else the outputs.
+template <typename T, typename I, int GATE, bool BWD, bool MAPS, int STAGES>
+__global__ void __launch_bounds__(32) recurrence_stream_kernel(const ScanArgs<T> p) {
+  constexpr int kArrays = stream_arrays<GATE, BWD, MAPS>();
+  constexpr int V = 16 / (int)sizeof(T), kLanes = 32 / V;  // lanes that copy a row of 32 values
+  extern __shared__ __align__(16) unsigned char smem[];
+  T* const ring = reinterpret_cast<T*>(smem);  // [STAGES][kArrays][kRows][32]
+  const int lane = threadIdx.x;
+  const int64_t item = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t total = (MAPS ? p.segments - 1 : p.segments) * p.columns;
+  const bool on = item < total;
+  const int64_t segment = on ? fdiv(item, p.by_columns) : 0, col = on ? item - segment * p.columns : 0;
+  const int64_t s0 = segment * p.steps;
+  const int64_t n = on ? min(p.steps, p.length - s0) : 0;  // this lane's steps
+  const I base = (I)column_base(p, col), step = (I)p.inner;
+  // Row r of the walk is chain step s0 + r, or from the segment's end s0 + n - 1 - r.
+  constexpr bool kUp = BWD == MAPS;  // memory offsets grow along the walk
+  const I first = element<BWD>(p, base, MAPS ? s0 + n - 1 : s0);
+  // What this lane copies: its own column value by value, or 16 bytes of the
+  // column pack of lane (lane % kLanes) * V.
+  const bool wide = p.wide;
+  const int source = wide ? lane % kLanes * V : lane;
+  const I from = (I)__shfl_sync(0xffffffffu, first, source);
+  const int64_t count = __shfl_sync(0xffffffffu, n, source);
+  const int row0 = wide ? lane / kLanes : 0, rows = wide ? V : 1;
+  // Where backward's h[t - 1] of the last step is the state, nothing is copied.
+  const int64_t zero = BWD && !MAPS ? p.length - 1 - s0 : -1;  // the row of t = 0, if it is one of this lane's
+  const int64_t from_zero = BWD && !MAPS ? __shfl_sync(0xffffffffu, zero, source) : -1;
+  int64_t most = n;  // the longest of the warp
 #pragma unroll
-    for (int i = 1; i < L; ++i) {
-      P *= (double)st.coefficient(i);
-      H = fma(st.coefficient(i), H, st.input(i));
-    }
-    map = make_double2(P, (double)H);
-  }
-  double2 before = make_double2(1.0, 0.0);
-  for (int k = 1; k < pieces; k <<= 1) {
-    // Inclusive scan over the pieces, each composition in a fixed order.
-    double2 prev;
-    prev.x = __shfl_up_sync(0xffffffffu, map.x, k * width);
-    prev.y = __shfl_up_sync(0xffffffffu, map.y, k * width);
-    if (piece >= k) map = compose(prev, map);
-  }
-  if (pieces > 1) {
-    double2 prev;
-    prev.x = __shfl_up_sync(0xffffffffu, map.x, width);
-    prev.y = __shfl_up_sync(0xffffffffu, map.y, width);
-    if (piece > 0) before = prev;
-  }
-  if (piece == pieces - 1) warp_map[warp][lc] = map;
-  __syncthreads();
+  for (int o = 16; o > 0; o >>= 1) most = max(most, (int64_t)__shfl_xor_sync(0xffffffffu, most, o));
+  const int64_t stages = (most + kRows - 1) / kRows;
 
-  const unsigned groups = (p.chunks + kGroup - 1) / kGroup;
-  unsigned* const chunk_flag = p.words + kFlagWords + (size_t)tile * p.chunks;
-  unsigned* const group_flag = p.words + kFlagWords + (size_t)p.tiles * p.chunks + (size_t)tile * groups;
-  const unsigned group = chunk / kGroup, place = chunk % kGroup;
-  const bool behind = chunk + 1 < p.chunks;  // some chunk waits for this one
-  const bool writer = piece == 0 && on;
-  double2 all;  // the block's map (warp 0)
-  if (warp == 0) {
-    all = warp_map[0][lc];
-    for (int w = 1; w < kWarps; ++w) all = compose(all, warp_map[w][lc]);
-    if (behind && place != kGroup - 1) {
-      if (writer) __stcg(p.maps + (int64_t)chunk * p.columns + col, all);
-      __syncwarp();
-      if (lane == 0) {
-        __threadfence();
-        store_release(chunk_flag + chunk, epoch);
+  auto copy = [&](int64_t k) {
+    if (k < stages) {
+      T* const to = ring + (size_t)(k % STAGES) * kArrays * kRows * 32 + source;
+      I e = kUp ? (I)(from + (I)(k * kRows + row0) * step) : (I)(from - (I)(k * kRows + row0) * step);
+      const I de = kUp ? (I)((I)rows * step) : (I)(I(0) - (I)rows * step);
+      auto put = [&](int array, int r, const T* src, bool there) {
+        T* const q = to + (array * kRows + r) * 32;
+        if (wide) copy_async<16>(q, there ? src : p.a, there);
+        else copy_async<(int)sizeof(T)>(q, there ? src : p.a, there);
+      };
+      auto some = [&](int r) {
+        const bool there = k * kRows + r < count;
+        put(0, r, at(p.a, e), there);
+        put(1, r, at(BWD ? p.dh : p.b, e), there);
+        if constexpr (kArrays > 2) put(2, r, at(p.h, (I)(e - step)), there && k * kRows + r != from_zero);
+        if constexpr (kArrays > 3) put(3, r, at(p.b, e), there);
+        e += de;
+      };
+      if (wide) {
+#pragma unroll
+        for (int r = 0; r < kRows / V; ++r) some(row0 + r * V);
+      } else {
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) some(r);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int k = 0; k < STAGES - 1; ++k) copy(k);
+
+  // The value before the segment.
+  T x = T(0);
+  if constexpr (!MAPS) {
+    if (on) {
+      if (p.starts) {
+        x = (T)p.starts[item];
+      } else {
+        double v = p.start ? (double)p.start[col] : 0.0;
+        for (int64_t k = 0; k < segment; k += 8) {
+          double2 m[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (k + i < segment) m[i] = p.maps[(k + i) * p.columns + col];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (k + i < segment) v = apply(m[i], v);
+        }
+        x = (T)v;
       }
     }
   }
-  // The maps of the group's chunks before this one, a warp for each (so that
-  // their latencies overlap), and the value at the end of the group before.
-  for (unsigned k = warp; k < place; k += kWarps) {
-    if (lane == 0) wait_flag(chunk_flag + group * kGroup + k, epoch, p.err);
-    __syncwarp();
-    if (writer) earlier[k][lc] = __ldcg(p.maps + (int64_t)(group * kGroup + k) * p.columns + col);
+  // Backward: the coefficient of the next step, at first that of the segment's
+  // first one: the gate at t + 1, or 1 at the end of the sequence.
+  T c = T(1);
+  const T state = BWD && !MAPS && on && p.state ? __ldg(p.state + col) : T(0);
+  if constexpr (BWD && !MAPS) {
+    if (on && s0 > 0) {
+      T unused = T(0);
+      c = Step<T, GATE, true>::gate(__ldg(at(p.a, (I)(first + step))), &unused);
+    }
   }
-  if (warp == kWarps - 1) {
-    double x = 0.0;
-    if (group == 0) {
-      if (p.start && on) x = (double)p.start[col];
+  double P = 1.0, H = 0.0;
+  T later = T(0);  // backward maps: dh of the chain step behind the one at hand
+  I e = first;
+  for (int64_t k = 0; k < stages; ++k) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncwarp();  // every lane's copies are there, and every lane has left the stage that is filled next
+    copy(k + STAGES - 1);
+    const T* const q = ring + (size_t)(k % STAGES) * kArrays * kRows * 32 + lane;
+    const int64_t left = n - k * kRows;
+    auto one = [&](int i) {
+      const T a = q[i * 32], b = q[(kRows + i) * 32];
+      if constexpr (MAPS && !BWD) {
+        T c1, u;
+        Step<T, GATE, false>::operands(a, b, &c1, &u);
+        H = u == T(0) ? H : fma(P, (double)u, H);  // 0 stays 0 behind an overflowed product
+        P *= (double)c1;
+      } else if constexpr (MAPS) {
+        // Walking towards the chain's start: the gate of a step is the
+        // coefficient of the step behind it, which came before.
+        T unused = T(0);
+        if (k * kRows + i > 0) P *= (double)Step<T, GATE, true>::gate(a, &unused);
+        H = b == T(0) ? H : fma(P, (double)b, H);
+      } else if constexpr (!BWD) {
+        T c1, u;
+        Step<T, GATE, false>::operands(a, b, &c1, &u);
+        x = fma(c1, x, u);
+        *at(p.out0, e) = x;
+        e += step;
+      } else {
+        x = fma(c, x, b);
+        T rest = T(0), da, db;
+        c = Step<T, GATE, true>::gate(a, &rest);
+        T before = q[(2 * kRows + i) * 32], put = T(0);
+        if (k * kRows + i == zero) before = state;
+        if constexpr (kArrays > 3) put = q[(3 * kRows + i) * 32];
+        Step<T, GATE, true>::outputs(x, c, rest, before, put, &da, &db);
+        *at(p.out1, e) = db;
+        *at(p.out0, e) = da;
+        e -= step;
+      }
+    };
+    if (left >= kRows) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) one(i);
     } else {
-      if (lane == 0) wait_flag(group_flag + group - 1, epoch, p.err);
-      __syncwarp();
-      if (on) x = __ldcg(p.ends + (int64_t)(group - 1) * p.columns + col);
-    }
-    if (piece == 0) carry[lc] = x;
-  }
-  __syncthreads();
-  double x = carry[lc];
-  for (unsigned k = 0; k < place; ++k) x = apply(earlier[k][lc], x);
-  if (warp == 0 && behind && place == kGroup - 1) {
-    if (writer) __stcg(p.ends + (int64_t)group * p.columns + col, apply(all, x));
-    __syncwarp();
-    if (lane == 0) {
-      __threadfence();
-      store_release(group_flag + group, epoch);
+      for (int i = 0; i < left; ++i) one(i);
     }
   }
-  for (int w = 0; w < warp; ++w) x = apply(warp_map[w][lc], x);
-  x = apply(before, x);
-  if (on && s0 < p.length) st.run(p, base, col, s0, (T)x);
-
-  if (threadIdx.x == 0) finish_words(p.words, epoch, p.tiles * p.chunks);
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (!on) return;
+  if constexpr (MAPS) {
+    if constexpr (BWD) {
+      // The first step's own coefficient.
+      if (s0 > 0) {
+        T unused = T(0);
+        const T a = __ldg(at(p.a, (I)(element<true>(p, base, s0) + step)));
+        P *= (double)Step<T, GATE, true>::gate(a, &unused);
+      }
+    }
+    p.maps[item] = make_double2(P, H);
+  } else if (p.last && s0 + n == p.length) {
+    p.last[col] = BWD ? c * x : x;
+  }
 }
 
-template <typename T, int GATE, bool BWD>
+// The value before each segment of a column, where segments are many: a warp
+// per column, its lanes composing consecutive runs of maps.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) recurrence_starts_kernel(const ScanArgs<T> p) {
+  const int64_t col = (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+  if (col >= p.columns) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t run = (p.segments + 31) / 32, k0 = lane * run, k1 = min(p.segments, k0 + run);
+  double2 map = make_double2(1.0, 0.0);
+#pragma unroll 4
+  for (int64_t k = k0; k < k1 && k < p.segments - 1; ++k) map = compose(map, p.maps[k * p.columns + col]);
+  // Over the lanes, in order.
+  double x = p.start ? (double)p.start[col] : 0.0, mine = x;
+  for (int l = 0; l < 31; ++l) {
+    double2 m;
+    m.x = __shfl_sync(0xffffffffu, map.x, l);
+    m.y = __shfl_sync(0xffffffffu, map.y, l);
+    x = apply(m, x);
+    if (lane == l + 1) mine = x;
+  }
+  for (int64_t k = k0; k < k1; ++k) {
+    p.starts[k * p.columns + col] = mine;
+    if (k < p.segments - 1) mine = apply(p.maps[k * p.columns + col], mine);
+  }
+}
+
+#ifndef PB_ST
+#define PB_ST 5
+#define PB_LANES 12288
+#endif
+template <typename T, typename I, int GATE, bool BWD, bool MAPS>
+int launch_stream(Device* d, const ScanArgs<T>& p) {
+  constexpr int kArrays = stream_arrays<GATE, BWD, MAPS>();
+  constexpr int STAGES = kArrays == 2 ? PB_ST : kArrays == 3 ? PB_ST - 1 : PB_ST - 2;
+  constexpr size_t bytes = sizeof(T) * STAGES * kArrays * kRows * 32;
+  const void* kernel = (const void*)recurrence_stream_kernel<T, I, GATE, BWD, MAPS, STAGES>;
+  PB_CHECK(allow_smem(d, kernel, bytes));
+  const int64_t warps = ceil_div((MAPS ? p.segments - 1 : p.segments) * p.columns, (int64_t)32);
+  recurrence_stream_kernel<T, I, GATE, BWD, MAPS, STAGES><<<(unsigned)warps, 32, bytes, d->stream>>>(p);
+  PB_LAUNCHED(d);
+  return PB_OK;
+}
+
+template <typename T, typename I, int GATE, bool BWD>
 int launch(Device* d, ScanArgs<T>& p) {
-  // Steps per thread: what keeps the registers of one thread near 64.
-  constexpr int L = BWD ? 8 : sizeof(T) == 4 ? 16 : 8;
-  int lanes = 0;
-  while (lanes < 5 && (int64_t(1) << lanes) < p.columns) ++lanes;
-  const int64_t tiles = ceil_div(p.columns, int64_t(1) << lanes);
-  const int64_t chunks = ceil_div(p.length, (int64_t)(kWarps * L) << (5 - lanes));
-  const int64_t groups = ceil_div(chunks, (int64_t)kGroup);
-  const bool cut = p.length > 2 * L && p.columns < (int64_t)d->sm_count * 1024 &&
-                   tiles * (chunks + groups) < (int64_t(1) << 26);
-  if (cut) {
-    void* ws;
-    const size_t maps = (size_t)chunks * p.columns, ends = (size_t)groups * p.columns;
-    PB_CHECK(scratch(d, maps * sizeof(double2) + ends * sizeof(double), &ws));
-    p.maps = static_cast<double2*>(ws);
-    p.ends = reinterpret_cast<double*>(p.maps + maps);
-    PB_CHECK(epoch_words(d, kFlagWords + (size_t)(tiles * (chunks + groups)), &p.words));
-    p.lanes_log2 = lanes;
-    p.tiles = (unsigned)tiles;
-    p.chunks = (unsigned)chunks;
-    p.err = d->err_dev;
+  // Lanes that keep HBM busy, and the columns from which the direct kernel does.
+  constexpr int64_t kEnough = PB_LANES, kMany = 131072;
+  if (p.length <= 2 * kRows || p.columns >= kMany) {
+    const int64_t blocks = ceil_div(p.columns, (int64_t)kThreads);
+    if (blocks > INT32_MAX) PB_FAIL(PB_ERR_UNSUPPORTED, "recurrence over more than 2^39 columns");
     PB_CHECK(kt_begin(d));
-    recurrence_chunks_kernel<T, GATE, BWD, L><<<(unsigned)(tiles * chunks), kThreads, 0, d->stream>>>(p);
+    recurrence_columns_kernel<T, I, GATE, BWD><<<(unsigned)blocks, kThreads, 0, d->stream>>>(p);
     PB_LAUNCHED(d);
     return kt_end(d);
   }
-  const int64_t blocks = ceil_div(p.columns, (int64_t)kThreads);
-  if (blocks > INT32_MAX) PB_FAIL(PB_ERR_UNSUPPORTED, "recurrence over more than 2^39 columns");
+  constexpr int V = 16 / (int)sizeof(T);
+  p.wide = p.inner % V == 0 && (((uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.h | (uintptr_t)p.dh) & 15) == 0;
+  p.by_columns = make_fastdiv(p.columns);
+  int64_t segments = p.columns >= kEnough * 2 / 3 ? 1 : ceil_div(kEnough * 3 / 2, p.columns);
+  const int64_t most = ceil_div(p.length, (int64_t)4 * kRows);
+  if (segments > most) segments = most;
+  p.steps = ceil_div(p.length, segments);
+  p.segments = ceil_div(p.length, p.steps);
+  if (p.segments > 1) {
+    void* ws;
+    const size_t cells = (size_t)p.segments * p.columns;
+    // Lanes that take their start from `state` must not meet the one that writes
+    // `final` over it: then the starts are formed first, too.
+    const bool starts = p.segments > kInlineMaps || (p.last && p.last == p.start);
+    PB_CHECK(scratch(d, cells * (sizeof(double2) + (starts ? sizeof(double) : 0)), &ws));
+    p.maps = static_cast<double2*>(ws);
+    p.starts = starts ? reinterpret_cast<double*>(p.maps + cells) : nullptr;
+  }
   PB_CHECK(kt_begin(d));
-  recurrence_columns_kernel<T, GATE, BWD, 8><<<(unsigned)blocks, kThreads, 0, d->stream>>>(p);
-  PB_LAUNCHED(d);
+  if (p.segments > 1) {
+    PB_CHECK((launch_stream<T, I, GATE, BWD, true>(d, p)));
+    if (p.starts) {
+      recurrence_starts_kernel<T><<<(unsigned)ceil_div(p.columns, (int64_t)(kThreads / 32)), kThreads, 0, d->stream>>>(p);
+      PB_LAUNCHED(d);
+    }
+  }
+  PB_CHECK((launch_stream<T, I, GATE, BWD, false>(d, p)));
   return kt_end(d);
 }
 
 template <typename T, bool BWD>
-int launch_gate(Device* d, int gate, ScanArgs<T> p) {
-  return gate == PB_GATE_SIGMOID ? launch<T, PB_GATE_SIGMOID, BWD>(d, p) : launch<T, PB_GATE_LINEAR, BWD>(d, p);
+int launch_gate(Device* d, int gate, ScanArgs<T> p, size_t bytes) {
+  const bool narrow = bytes < (size_t(1) << 32);
+  if (gate == PB_GATE_SIGMOID)
+    return narrow ? launch<T, uint32_t, PB_GATE_SIGMOID, BWD>(d, p) : launch<T, int64_t, PB_GATE_SIGMOID, BWD>(d, p);
+  return narrow ? launch<T, uint32_t, PB_GATE_LINEAR, BWD>(d, p) : launch<T, int64_t, PB_GATE_LINEAR, BWD>(d, p);
 }
 
 // Checks common to both directions; the array's bytes and those of a state.
@@ -383,6 +482,7 @@ ScanArgs<T> make_args(int64_t outer, int64_t length, int64_t inner, const void* 
   p.last = static_cast<T*>(last);
   p.length = length;
   p.inner = inner;
+  p.by_inner = make_fastdiv(inner);
   p.columns = outer * inner;
   return p;
 }
@@ -408,9 +508,9 @@ int pb_recurrence(pb_ctx* ctx, int dev, int dtype, int gate, int64_t outer, int6
   PB_CHECK(enter(ctx, dev, &d));
   if (dtype == PB_F32)
     return launch_gate<float, false>(d, gate, make_args<float, false>(outer, length, inner, a, b, nullptr, nullptr,
-                                                                      state, nullptr, h, nullptr, final));
+                                                                      state, nullptr, h, nullptr, final), bytes);
   return launch_gate<double, false>(d, gate, make_args<double, false>(outer, length, inner, a, b, nullptr, nullptr,
-                                                                      state, nullptr, h, nullptr, final));
+                                                                      state, nullptr, h, nullptr, final), bytes);
 }
 
 int pb_recurrence_backward(pb_ctx* ctx, int dev, int dtype, int gate, int64_t outer, int64_t length, int64_t inner,
@@ -429,9 +529,9 @@ int pb_recurrence_backward(pb_ctx* ctx, int dev, int dtype, int gate, int64_t ou
   PB_CHECK(enter(ctx, dev, &d));
   if (dtype == PB_F32)
     return launch_gate<float, true>(d, gate, make_args<float, true>(outer, length, inner, a, b, h, dh, dfinal, state,
-                                                                    da, db, dstate));
+                                                                    da, db, dstate), bytes);
   return launch_gate<double, true>(d, gate, make_args<double, true>(outer, length, inner, a, b, h, dh, dfinal, state,
-                                                                    da, db, dstate));
+                                                                    da, db, dstate), bytes);
 }
 
 }  // extern "C"
