@@ -230,9 +230,12 @@ __global__ void __launch_bounds__(32) recurrence_stream_kernel(const ScanArgs<T>
   for (int o = 16; o > 0; o >>= 1) most = max(most, (int64_t)__shfl_xor_sync(0xffffffffu, most, o));
   const int64_t stages = (most + kRows - 1) / kRows;
 
+  constexpr int kStage = kArrays * kRows * 32;  // values
+  int copy_slot = 0, slot = 0;                  // where the next copy goes, and the stage at hand is
   auto copy = [&](int64_t k) {
     if (k < stages) {
-      T* const to = ring + (size_t)(k % STAGES) * kArrays * kRows * 32 + source;
+      T* const to = ring + copy_slot * kStage + source;
+      copy_slot = copy_slot + 1 == STAGES ? 0 : copy_slot + 1;
       I e = kUp ? (I)(from + (I)(k * kRows + row0) * step) : (I)(from - (I)(k * kRows + row0) * step);
       const I de = kUp ? (I)((I)rows * step) : (I)(I(0) - (I)rows * step);
       auto put = [&](int array, int r, const T* src, bool there) {
@@ -298,7 +301,8 @@ __global__ void __launch_bounds__(32) recurrence_stream_kernel(const ScanArgs<T>
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();  // every lane's copies are there, and every lane has left the stage that is filled next
     copy(k + STAGES - 1);
-    const T* const q = ring + (size_t)(k % STAGES) * kArrays * kRows * 32 + lane;
+    const T* const q = ring + slot * kStage + lane;
+    slot = slot + 1 == STAGES ? 0 : slot + 1;
     const int64_t left = n - k * kRows;
     auto one = [&](int i) {
       const T a = q[i * 32], b = q[(kRows + i) * 32];
@@ -382,14 +386,14 @@ __global__ void __launch_bounds__(kThreads) recurrence_starts_kernel(const ScanA
   }
 }
 
-#ifndef PB_ST
-#define PB_ST 5
-#define PB_LANES 12288
-#endif
 template <typename T, typename I, int GATE, bool BWD, bool MAPS>
 int launch_stream(Device* d, const ScanArgs<T>& p) {
   constexpr int kArrays = stream_arrays<GATE, BWD, MAPS>();
-  constexpr int STAGES = kArrays == 2 ? PB_ST : kArrays == 3 ? PB_ST - 1 : PB_ST - 2;
+  // What is on its way for a warp (float32): 32 KiB forward, 18 to 24 in
+  // the others, of which more fit beside each other.  8 x 4096 x 2048: forward
+  // 127 us with eight stages, 132 with five, 139 with four; backward 249 with
+  // three of four arrays, 300 with six, 334 with two.
+  constexpr int STAGES = MAPS ? 5 : kArrays == 2 ? 8 : kArrays == 3 ? 4 : 3;
   constexpr size_t bytes = sizeof(T) * STAGES * kArrays * kRows * 32;
   const void* kernel = (const void*)recurrence_stream_kernel<T, I, GATE, BWD, MAPS, STAGES>;
   PB_CHECK(allow_smem(d, kernel, bytes));
@@ -401,8 +405,11 @@ int launch_stream(Device* d, const ScanArgs<T>& p) {
 
 template <typename T, typename I, int GATE, bool BWD>
 int launch(Device* d, ScanArgs<T>& p) {
-  // Lanes that keep HBM busy, and the columns from which the direct kernel does.
-  constexpr int64_t kEnough = PB_LANES, kMany = 131072;
+  // Columns from which uncut chains keep HBM busy, the lanes of cut ones (16381 x 1024
+  // float32: 57 us with 18432 lanes, 61 with 13500 or 36864; 3 x 1000 x 515 float64
+  // backward: 25 us with 13500 lanes, 29 with 18432), and the columns from which the
+  // direct kernel has enough threads.
+  constexpr int64_t kEnough = 8192, kLanes = sizeof(T) == 4 ? 18432 : 13500, kMany = 131072;
   if (p.length <= 2 * kRows || p.columns >= kMany) {
     const int64_t blocks = ceil_div(p.columns, (int64_t)kThreads);
     if (blocks > INT32_MAX) PB_FAIL(PB_ERR_UNSUPPORTED, "recurrence over more than 2^39 columns");
@@ -414,7 +421,7 @@ int launch(Device* d, ScanArgs<T>& p) {
   constexpr int V = 16 / (int)sizeof(T);
   p.wide = p.inner % V == 0 && (((uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.h | (uintptr_t)p.dh) & 15) == 0;
   p.by_columns = make_fastdiv(p.columns);
-  int64_t segments = p.columns >= kEnough * 2 / 3 ? 1 : ceil_div(kEnough * 3 / 2, p.columns);
+  int64_t segments = p.columns >= kEnough ? 1 : ceil_div(kLanes, p.columns);
   const int64_t most = ceil_div(p.length, (int64_t)4 * kRows);
   if (segments > most) segments = most;
   p.steps = ceil_div(p.length, segments);

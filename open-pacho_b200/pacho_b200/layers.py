@@ -37,7 +37,7 @@ def _context(x, what):
     backend = getattr(getattr(x, "_data", None), "backend", None)
     if not isinstance(backend, B200Backend):
         raise TypeError(f"{what} takes arrays of the b200 backend, not {type(x).__name__}")
-    dtype = np.dtype(x.dtype)
+    dtype = x.dtype
     code = _FLOATS.get(dtype)
     if code is None:
         raise _exc.UnsupportedDtypeError(f"{what} requires float32 or float64, not {dtype}")
@@ -50,9 +50,13 @@ def _pointer(name, x, shape, dtype, backend):
     if x is None:
         return None
     data = x._data
+    # The usual case in three comparisons: a call's time on the host is what its
+    # smallest sizes take.
+    if data.backend is backend and x.shape == shape and (x.dtype is dtype or x.dtype == dtype):
+        return data.ptr
     if data.backend is not backend:
         raise _exc.BackendMismatchError(f"{name} belongs to another backend")
-    if x.shape != shape and tuple(x.shape) != shape:
+    if tuple(x.shape) != shape:
         raise ValueError(f"{name} has shape {tuple(x.shape)}, expected {shape}")
     if x.dtype != dtype:
         raise ValueError(f"{name} has dtype {x.dtype}, expected {dtype}")
@@ -75,24 +79,18 @@ def _outputs(out, count, what):
     return out
 
 
-def _gate(gate):
+def _choice(what, choices, value):
     try:
-        return _lib.GATES[gate]
+        return choices[value]
     except (KeyError, TypeError):
-        raise ValueError(f"unknown gate {gate!r}: {', '.join(map(repr, _lib.GATES))}") from None
-
-
-def _activation(activation):
-    try:
-        return _lib.ACTIVATIONS[activation]
-    except (KeyError, TypeError):
-        raise ValueError(f"unknown activation {activation!r}: "
-                         f"{', '.join(map(repr, _lib.ACTIVATIONS))}") from None
+        raise ValueError(f"unknown {what} {value!r}: {', '.join(map(repr, choices))}") from None
 
 
 def _axis_view(shape, axis, what):
     """(outer, length, inner, shape without the axis)."""
     ndim = len(shape)
+    if ndim == 3 and (axis == -2 or axis == 1):
+        return shape[0], shape[1], shape[2], (shape[0], shape[2])
     if not -ndim <= axis < ndim:
         raise ValueError(f"{what}: axis {axis} is out of range for {ndim} dimensions")
     axis %= ndim
@@ -112,9 +110,9 @@ def linear_recurrence(a, b, *, state=None, gate="linear", axis=-2, out=None, fin
     Returns h (``out`` if given)."""
     backend, dtype, code = _context(a, "linear_recurrence")
     shape = tuple(a.shape)
-    mode = _gate(gate)
+    mode = _choice("gate", _lib.GATES, gate)
     outer, length, inner, rest = _axis_view(shape, axis, "linear_recurrence")
-    pa = _pointer("a", a, shape, dtype, backend)
+    pa = a._data.ptr
     pb = _pointer("b", b, shape, dtype, backend)
     ps = _pointer("state", state, rest, dtype, backend)
     pf = _pointer("final", final, rest, dtype, backend)
@@ -133,11 +131,11 @@ def linear_recurrence_backward(a, b, h, dh, *, state=None, dfinal=None, gate="li
     None with ``gate="linear"``, whose gradients do not depend on it."""
     backend, dtype, code = _context(a, "linear_recurrence_backward")
     shape = tuple(a.shape)
-    mode = _gate(gate)
+    mode = _choice("gate", _lib.GATES, gate)
     outer, length, inner, rest = _axis_view(shape, axis, "linear_recurrence_backward")
     if b is None and mode != _lib.GATES["linear"]:
         raise ValueError(f"the gradients of gate={gate!r} need b")
-    pa = _pointer("a", a, shape, dtype, backend)
+    pa = a._data.ptr
     pb = _pointer("b", b, shape, dtype, backend)
     ph = _pointer("h", h, shape, dtype, backend)
     pg = _pointer("dh", dh, shape, dtype, backend)
@@ -163,7 +161,7 @@ def _norm_view(x, groups, what):
     groups = int(groups)
     if groups < 1 or shape[-1] % groups:
         raise ValueError(f"{what}: {shape[-1]} channels do not divide into {groups} groups")
-    return shape[0], prod(shape[1:-1]), shape[-1], groups
+    return shape[0], shape[1] if len(shape) == 3 else prod(shape[1:-1]), shape[-1], groups
 
 
 def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, out=None):
@@ -176,15 +174,16 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
     ``(tokens, C)`` with a group per head.  Returns ``(y, mean, rstd)``, the
     statistics ``(N, groups)`` for the backward pass; ``out`` takes the three."""
     backend, dtype, code = _context(x, "group_norm")
-    act = _activation(activation)
+    act = _choice("activation", _lib.ACTIVATIONS, activation)
     n, s, c, groups = _norm_view(x, groups, "group_norm")
-    px = _pointer("x", x, tuple(x.shape), dtype, backend)
+    shape = tuple(x.shape)
+    px = x._data.ptr
     pw = _pointer("weight", weight, (c,), dtype, backend)
     pb = _pointer("bias", bias, (c,), dtype, backend)
     y, mean, rstd = _outputs(out, 3, "group_norm")
     with backend._lock:
         backend._require_open()
-        y, py = _output("y", y, tuple(x.shape), dtype, backend, x)
+        y, py = _output("y", y, shape, dtype, backend, x)
         mean, pm = _output("mean", mean, (n, groups), dtype, backend, x)
         rstd, pr = _output("rstd", rstd, (n, groups), dtype, backend, x)
         backend._check(backend._lib.pb_group_norm(backend._ctx, 0, code, act, n, s, c, groups, float(eps),
@@ -197,10 +196,10 @@ def group_norm_backward(dy, x, groups, mean, rstd, weight=None, bias=None, *, ac
     ``x``, ``weight``, ``bias`` and activation, with the ``mean`` and ``rstd`` it
     returned.  ``dweight`` is None without a weight, ``dbias`` without a bias."""
     backend, dtype, code = _context(x, "group_norm_backward")
-    act = _activation(activation)
+    act = _choice("activation", _lib.ACTIVATIONS, activation)
     n, s, c, groups = _norm_view(x, groups, "group_norm_backward")
     shape = tuple(x.shape)
-    px = _pointer("x", x, shape, dtype, backend)
+    px = x._data.ptr
     pd = _pointer("dy", dy, shape, dtype, backend)
     pm = _pointer("mean", mean, (n, groups), dtype, backend)
     pr = _pointer("rstd", rstd, (n, groups), dtype, backend)
@@ -245,12 +244,12 @@ class AdamW:
             raise ValueError("betas are two numbers")
         self.steps = int(steps)
         self._shapes = [tuple(p.shape) for p in self.params]
-        count = len(self.params)
+        self._pointers = C.c_void_p * len(self.params)
         self._p = self._table("params", self.params)
         self.exp_avg = self._moment("exp_avg", exp_avg)
         self.exp_avg_sq = self._moment("exp_avg_sq", exp_avg_sq)
         self._m, self._v = self._table("exp_avg", self.exp_avg), self._table("exp_avg_sq", self.exp_avg_sq)
-        self._sizes = (C.c_int64 * count)(*[prod(s) for s in self._shapes])
+        self._sizes = (C.c_int64 * len(self.params))(*[prod(s) for s in self._shapes])
 
     def _moment(self, name, given):
         if given is not None:
@@ -264,7 +263,11 @@ class AdamW:
         if len(arrays) != len(self._shapes):
             raise ValueError(f"{name}: {len(arrays)} arrays for {len(self._shapes)} parameters")
         b, dtype = self._backend, self._dtype
-        return (C.c_void_p * len(arrays))(*[_pointer(name, x, s, dtype, b) for x, s in zip(arrays, self._shapes)])
+        pointers = [x._data.ptr for x, s in zip(arrays, self._shapes)
+                    if x._data.backend is b and x.dtype is dtype and x.shape == s]
+        if len(pointers) != len(arrays):  # one is not quite so: checked one by one
+            pointers = [_pointer(name, x, s, dtype, b) for x, s in zip(arrays, self._shapes)]
+        return self._pointers(*pointers)
 
     def step(self, grads, *, grad_scale=None):
         """One step with a gradient array per parameter (shape and dtype of

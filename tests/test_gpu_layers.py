@@ -542,3 +542,25 @@ def test_serving_token_by_token_gives_the_whole_sequence(b200):
                              gate="sigmoid", out=out)
         rows.append(out.numpy())
     close(np.concatenate(rows, 1), *want, np.float32, "tokens")
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_recurrence_in_several_windows(b200, dtype):
+    """Few columns, more operands than fit L2: the chain is read in windows."""
+    n, c = (300001, 32) if dtype == np.float32 else (150001, 32)
+    rng = np.random.default_rng(12)
+    a = rng.uniform(0.5, 1.0, (1, n, c)).astype(dtype)
+    b = rng.standard_normal((1, n, c)).astype(dtype)
+    state = rng.standard_normal((1, c)).astype(dtype)
+    keep = up(b200, state)
+    da, db = up(b200, a), up(b200, b)
+    h = pb.linear_recurrence(da, db, state=keep, final=keep)
+    got = h.numpy()
+    want, bound = ref.recurrence(a, b, state, "linear", ref.U[np.dtype(dtype)])
+    close(got, want, bound, dtype, "h")
+    assert keep.numpy().tobytes() == got[:, -1].tobytes()
+    dh = rng.standard_normal(a.shape).astype(dtype)
+    grads = pb.linear_recurrence_backward(da, db, h, up(b200, dh), state=up(b200, state))
+    want, bounds = ref.recurrence_backward(a, b, got, dh, state, None, "linear", ref.U[np.dtype(dtype)])
+    for name, g, w, e in zip(("da", "db", "dstate"), grads, want, bounds):
+        close(g.numpy(), w, e, dtype, name)
