@@ -22,8 +22,8 @@
 // neither over- nor underflows where a float32 recurrence does not.  Every
 // composition has a fixed order, so results do not depend on timing.
 //
-// Few steps, or more columns than fill the card: a thread per column reads
-// directly (recurrence_columns_kernel).
+// Few steps, or columns enough to fill the card with threads: a thread per column
+// reads directly (recurrence_columns_kernel).
 #include <type_traits>
 
 #include "pb_layers.cuh"
@@ -121,34 +121,35 @@ struct Step<T, GATE, true> {
 // issued together.
 template <typename T, typename I, int GATE, bool BWD>
 __global__ void __launch_bounds__(kThreads) recurrence_columns_kernel(const ScanArgs<T> p) {
-  constexpr int kAhead = 8;
+  constexpr int kAhead = 16;
   const int64_t col = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (col >= p.columns) return;
   const I base = (I)column_base(p, col), step = (I)p.inner;
   T x = p.start ? p.start[col] : T(0);
   T c = T(1);  // backward: the coefficient of the next step
-  for (int64_t s0 = 0; s0 < p.length; s0 += kAhead) {
-    const int left = (int)min((int64_t)kAhead, p.length - s0);
-    I e = element<BWD>(p, base, s0);
+  // kAhead steps (FULL), or the `left` last ones.
+  auto walk = [&](auto full, int64_t s0, int left) {
+    constexpr bool FULL = decltype(full)::value;
+    const I e = element<BWD>(p, base, s0);
     T a[kAhead], b[kAhead], g[BWD ? kAhead : 1], before[BWD ? kAhead : 1];
+    I q = e;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      a[i] = b[i] = T(0);
-      if (i < left) {
-        const I q = BWD ? (I)(e - (I)i * step) : (I)(e + (I)i * step);
+      if (FULL || i < left) {
         a[i] = __ldg(at(p.a, q));
         if (!BWD || GATE == PB_GATE_SIGMOID) b[i] = __ldg(at(p.b, q));
         if constexpr (BWD) {
           g[i] = __ldg(at(p.dh, q));
-          if (s0 + i + 1 < p.length) before[i] = __ldg(at(p.h, (I)(q - step)));
+          if (FULL || i + 1 < left) before[i] = __ldg(at(p.h, (I)(q - step)));
           else before[i] = p.state ? p.state[col] : T(0);
         }
+        q = BWD ? (I)(q - step) : (I)(q + step);
       }
     }
+    q = e;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      if (i < left) {
-        const I q = BWD ? (I)(e - (I)i * step) : (I)(e + (I)i * step);
+      if (FULL || i < left) {
         if constexpr (!BWD) {
           T u;
           Step<T, GATE, false>::operands(a[i], b[i], &c, &u);
@@ -162,9 +163,14 @@ __global__ void __launch_bounds__(kThreads) recurrence_columns_kernel(const Scan
           *at(p.out1, q) = db;
           *at(p.out0, q) = da;
         }
+        q = BWD ? (I)(q - step) : (I)(q + step);
       }
     }
-  }
+  };
+  // The last steps go apart: t = 0, whose h[t - 1] is the state, is among them.
+  int64_t s0 = 0;
+  for (; s0 + kAhead < p.length; s0 += kAhead) walk(std::true_type{}, s0, kAhead);
+  if (s0 < p.length) walk(std::false_type{}, s0, (int)(p.length - s0));
   if (p.last) p.last[col] = BWD ? c * x : x;
 }
 
@@ -187,6 +193,13 @@ __device__ __forceinline__ void copy_async(void* to, const void* from, bool ther
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(from), "r"(n) : "memory");
   else
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(s), "l"(from), "n"(BYTES), "r"(n) : "memory");
+}
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  const unsigned s = shared_address(to);
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(s), "l"(from), "n"(BYTES) : "memory");
 }
 
 // The operands of a stage: forward a, b; backward a, dh and, unless only maps
@@ -236,28 +249,37 @@ __global__ void __launch_bounds__(32) recurrence_stream_kernel(const ScanArgs<T>
     if (k < stages) {
       T* const to = ring + copy_slot * kStage + source;
       copy_slot = copy_slot + 1 == STAGES ? 0 : copy_slot + 1;
-      I e = kUp ? (I)(from + (I)(k * kRows + row0) * step) : (I)(from - (I)(k * kRows + row0) * step);
+      const I ahead = (I)(k * kRows + row0) * step;
+      I e = kUp ? (I)(from + ahead) : (I)(from - ahead);
       const I de = kUp ? (I)((I)rows * step) : (I)(I(0) - (I)rows * step);
-      auto put = [&](int array, int r, const T* src, bool there) {
-        T* const q = to + (array * kRows + r) * 32;
-        if (wide) copy_async<16>(q, there ? src : p.a, there);
-        else copy_async<(int)sizeof(T)>(q, there ? src : p.a, there);
-      };
-      auto some = [&](int r) {
-        const bool there = k * kRows + r < count;
-        put(0, r, at(p.a, e), there);
-        put(1, r, at(BWD ? p.dh : p.b, e), there);
-        if constexpr (kArrays > 2) put(2, r, at(p.h, (I)(e - step)), there && k * kRows + r != from_zero);
-        if constexpr (kArrays > 3) put(3, r, at(p.b, e), there);
+      const int64_t left = count - k * kRows, none = from_zero - k * kRows;
+      // A stage whose rows are all there needs no sizes; `bytes` of a copy else.
+      auto some = [&](auto whole, auto bytes, int r) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        constexpr int N = decltype(bytes)::value;
+        const bool there = WHOLE || r < left;
+        auto put = [&](int array, const T* src, bool now) {
+          T* const q = to + (array * kRows + r) * 32;
+          if constexpr (WHOLE) copy_async<N>(q, src);
+          else copy_async<N>(q, now ? src : p.a, now);
+        };
+        put(0, at(p.a, e), there);
+        put(1, at(BWD ? p.dh : p.b, e), there);
+        if constexpr (kArrays > 2) put(2, at(p.h, (I)(e - step)), there && r != none);
+        if constexpr (kArrays > 3) put(3, at(p.b, e), there);
         e += de;
       };
-      if (wide) {
+      auto all = [&](auto whole) {
+        if (wide) {
 #pragma unroll
-        for (int r = 0; r < kRows / V; ++r) some(row0 + r * V);
-      } else {
+          for (int r = 0; r < kRows / V; ++r) some(whole, std::integral_constant<int, 16>{}, row0 + r * V);
+        } else {
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) some(r);
-      }
+          for (int r = 0; r < kRows; ++r) some(whole, std::integral_constant<int, (int)sizeof(T)>{}, r);
+        }
+      };
+      if (__all_sync(0xffffffffu, left >= kRows && !(kArrays > 2 && none >= 0 && none < kRows))) all(std::true_type{});
+      else all(std::false_type{});
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -386,31 +408,48 @@ __global__ void __launch_bounds__(kThreads) recurrence_starts_kernel(const ScanA
   }
 }
 
-template <typename T, typename I, int GATE, bool BWD, bool MAPS>
-int launch_stream(Device* d, const ScanArgs<T>& p) {
-  constexpr int kArrays = stream_arrays<GATE, BWD, MAPS>();
-  // What is on its way for a warp (float32): 32 KiB forward, 18 to 24 in
-  // the others, of which more fit beside each other.  8 x 4096 x 2048: forward
-  // 127 us with eight stages, 132 with five, 139 with four; backward 249 with
-  // three of four arrays, 300 with six, 334 with two.
-  constexpr int STAGES = MAPS ? 5 : kArrays == 2 ? 8 : kArrays == 3 ? 4 : 3;
-  constexpr size_t bytes = sizeof(T) * STAGES * kArrays * kRows * 32;
-  const void* kernel = (const void*)recurrence_stream_kernel<T, I, GATE, BWD, MAPS, STAGES>;
-  PB_CHECK(allow_smem(d, kernel, bytes));
-  const int64_t warps = ceil_div((MAPS ? p.segments - 1 : p.segments) * p.columns, (int64_t)32);
+template <typename T, typename I, int GATE, bool BWD, bool MAPS, int STAGES>
+int launch_ring(Device* d, const ScanArgs<T>& p, int64_t warps) {
+  constexpr size_t bytes = sizeof(T) * STAGES * stream_arrays<GATE, BWD, MAPS>() * kRows * 32;
+  PB_CHECK(allow_smem(d, (const void*)recurrence_stream_kernel<T, I, GATE, BWD, MAPS, STAGES>, bytes));
   recurrence_stream_kernel<T, I, GATE, BWD, MAPS, STAGES><<<(unsigned)warps, 32, bytes, d->stream>>>(p);
   PB_LAUNCHED(d);
   return PB_OK;
+}
+
+template <typename T, typename I, int GATE, bool BWD, bool MAPS>
+int launch_stream(Device* d, const ScanArgs<T>& p) {
+  constexpr int kArrays = stream_arrays<GATE, BWD, MAPS>();
+  const int64_t warps = ceil_div((MAPS ? p.segments - 1 : p.segments) * p.columns, (int64_t)32);
+  // Few warps: what keeps HBM busy is on its way for each (float32: 32 KiB
+  // forward, 24 backward).  Many: less, so that more of them fit an SM.  8 x
+  // 4096 x 2048 float32, 512 warps: forward 127 us with eight stages, 139 with four;
+  // backward 249 with three of four arrays, 300 with six, 334 with two.
+  // 3 x 1000 x 515 float64 backward, 435 warps: 26 us with eight stages for the maps and
+  // four for the outputs, 29 with five and four, 30 with eight and six.
+  const int64_t per_sm = ceil_div(warps, (int64_t)d->sm_count);
+  if constexpr (kArrays == 2) {
+    if (per_sm > (sizeof(T) == 4 ? 6 : 3))
+      return launch_ring<T, I, GATE, BWD, MAPS, (sizeof(T) == 4 ? 5 : 3)>(d, p, warps);
+    return launch_ring<T, I, GATE, BWD, MAPS, 8>(d, p, warps);
+  } else {
+    return launch_ring<T, I, GATE, BWD, MAPS, (kArrays == 3 ? 4 : 3)>(d, p, warps);
+  }
 }
 
 template <typename T, typename I, int GATE, bool BWD>
 int launch(Device* d, ScanArgs<T>& p) {
   // Columns from which uncut chains keep HBM busy, the lanes of cut ones (16381 x 1024
   // float32: 57 us with 18432 lanes, 61 with 13500 or 36864; 3 x 1000 x 515 float64
-  // backward: 25 us with 13500 lanes, 29 with 18432), and the columns from which the
-  // direct kernel has enough threads.
-  constexpr int64_t kEnough = 8192, kLanes = sizeof(T) == 4 ? 18432 : 13500, kMany = 131072;
-  if (p.length <= 2 * kRows || p.columns >= kMany) {
+  // backward: 25 us with 13500 lanes, 29 with 18432).
+  constexpr int64_t kEnough = 8192, kLanes = sizeof(T) == 4 ? 18432 : 13500;
+  constexpr int V = 16 / (int)sizeof(T);
+  p.wide = p.inner % V == 0 && (((uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.h | (uintptr_t)p.dh) & 15) == 0;
+  // 16 x 1024 x 4096 float32: 133 us as streams, 157 directly; 32 x 512 x 4096: 153
+  // and 132; 30 x 500 x 4001 sigmoid (copies of one value): 218 and 131; 16 x 500 x
+  // 4096 float64 sigmoid: 174 and 138.
+  const int64_t many = sizeof(T) == 4 && p.wide ? 98304 : 49152;
+  if (p.length <= 2 * kRows || p.columns >= many) {
     const int64_t blocks = ceil_div(p.columns, (int64_t)kThreads);
     if (blocks > INT32_MAX) PB_FAIL(PB_ERR_UNSUPPORTED, "recurrence over more than 2^39 columns");
     PB_CHECK(kt_begin(d));
@@ -418,8 +457,6 @@ int launch(Device* d, ScanArgs<T>& p) {
     PB_LAUNCHED(d);
     return kt_end(d);
   }
-  constexpr int V = 16 / (int)sizeof(T);
-  p.wide = p.inner % V == 0 && (((uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.h | (uintptr_t)p.dh) & 15) == 0;
   p.by_columns = make_fastdiv(p.columns);
   int64_t segments = p.columns >= kEnough ? 1 : ceil_div(kLanes, p.columns);
   const int64_t most = ceil_div(p.length, (int64_t)4 * kRows);
