@@ -16,11 +16,11 @@
 // about one item per block.  The second read then finds the sample in L2
 // (up to about half of its 126 MB) while the next sample's first read keeps HBM busy.
 //
-// With one position (S = 1: a norm of each token) a group is a row of m
-// contiguous values, which fits into the registers of a part of a warp, a warp
-// or a block: one pass reads it, forms its sums and writes the result.  Such a
-// part of the block stays with one group and walks over the samples, so that
-// weight and bias stay in registers and the sums of dweight and dbias are its own.
+// A small group (all of one with S = 1, a norm of each token) fits into the
+// registers of a part of a warp, a warp or a block: one pass reads it, forms its
+// sums and writes the result.  Such a part of the block stays with one group and
+// walks over the samples, so that weight and bias stay in registers and the sums of
+// dweight and dbias are its own.
 #include "pb_layers.cuh"
 
 namespace pb {
@@ -48,15 +48,37 @@ struct NormArgs {
   double eps;
 };
 
+// Phi(z), the normal distribution's, and phi(z), its density.
+//
+// float32: Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26: erfc(x) =
+// (a1 t + ... + a5 t^5) e^(-x^2), t = 1 / (1 + p x), within 1.5e-7 for x >= 0; with x =
+// |z| / sqrt 2 the exponential is that of phi, and Phi is off by 7.5e-8 at most, little
+// more than a rounding of its largest values.  erfcf takes four times as long.
+__device__ __forceinline__ void normal(float z, float* Phi, float* phi) {
+  const float x = fabsf(z) * 0.70710678f;
+  const float e = exp2_unit(z * z * -0.72134752f);  // e^(-z^2 / 2)
+  const float t = reciprocal_unit(fmaf(0.3275911f, x, 1.0f));
+  float q = fmaf(1.061405429f, t, -1.453152027f);
+  q = fmaf(q, t, 1.421413741f);
+  q = fmaf(q, t, -0.284496736f);
+  q = fmaf(q, t, 0.254829592f);
+  const float tail = 0.5f * q * t * e;
+  *Phi = z < 0.0f ? tail : 1.0f - tail;
+  *phi = e * 0.39894228f;
+}
+__device__ __forceinline__ void normal(double z, double* Phi, double* phi) {
+  *Phi = 0.5 * erfc(z * -0.70710678118654752);  // accurate for negative z, where 1 + erf would cancel
+  *phi = exp(-0.5 * z * z) * 0.39894228040143268;
+}
+
 template <typename T, int ACT>
 __device__ __forceinline__ T activate(T z) {
   if constexpr (ACT == PB_ACT_RELU) return z < T(0) ? T(0) : z;
   if constexpr (ACT == PB_ACT_SILU) return z * sigmoid(z);
   if constexpr (ACT == PB_ACT_GELU) {
-    // z Phi(z) with Phi(z) = erfc(-z / sqrt 2) / 2, which keeps its relative
-    // accuracy for negative z where 1 + erf would cancel.
-    if constexpr (sizeof(T) == 4) return z * (0.5f * erfcf(z * -0.70710678118654752f));
-    else return z * (0.5 * erfc(z * -0.70710678118654752));
+    T Phi, phi;
+    normal(z, &Phi, &phi);
+    return z * Phi;
   }
   return z;
 }
@@ -69,9 +91,9 @@ __device__ __forceinline__ T slope(T z) {
     return fma(s * z, T(1) - s, s);
   }
   if constexpr (ACT == PB_ACT_GELU) {
-    const T phi = exp_of(T(-0.5) * z * z) * T(0.39894228040143268);
-    if constexpr (sizeof(T) == 4) return fmaf(z, phi, 0.5f * erfcf(z * -0.70710678118654752f));
-    else return fma(z, phi, 0.5 * erfc(z * -0.70710678118654752));
+    T Phi, phi;
+    normal(z, &Phi, &phi);
+    return fma(z, phi, Phi);
   }
   return T(1);
 }
@@ -240,18 +262,23 @@ __device__ __forceinline__ void sum_rows(const NormArgs<T>& p, const S& sums, in
   }
 }
 
-// Over the channels of each group.
+// Over the channels of each group: a thread each, or a warp where they are many.
 template <typename T, bool BWD>
 __device__ __forceinline__ void sum_groups(const NormArgs<T>& p, const double2* channels, double2* part) {
-  for (int64_t g = threadIdx.x; g < p.G; g += kThreads) {
+  const int64_t lanes = p.m <= 16 ? 1 : 32;
+  for (int64_t g = threadIdx.x / lanes; g < p.G; g += kThreads / lanes) {
     double2 t = make_double2(0.0, 0.0);
-    for (int64_t c = g * p.m; c < (g + 1) * p.m; ++c) {
+    for (int64_t c = g * p.m + threadIdx.x % lanes; c < (g + 1) * p.m; c += lanes) {
       const double2 v = channels[c];
       const double w = BWD && p.weight ? (double)__ldg(p.weight + c) : 1.0;
       t.x = fma(w, v.x, t.x);
       t.y = fma(w, v.y, t.y);
     }
-    part[g] = t;
+    for (int o = (int)lanes / 2; o > 0; o >>= 1) {
+      t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
+      t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
+    }
+    if (threadIdx.x % lanes == 0) part[g] = t;
   }
 }
 
@@ -721,19 +748,20 @@ __device__ __forceinline__ T slope(int act, T z) {
 // each of them and in a fixed order.
 template <int LANES>
 __device__ __forceinline__ double2 row_sum(double2 t) {
+  constexpr int kRowWarps = LANES / 32;
 #pragma unroll
   for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) {
     t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
     t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
   }
   if constexpr (LANES > 32) {
-    __shared__ double2 part[kWarps];
+    __shared__ double2 part[kRowWarps];
     __syncthreads();  // the last use of `part` is over
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = t;
     __syncthreads();
     t = part[0];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) {
+    for (int w = 1; w < kRowWarps; ++w) {
       t.x += part[w].x;
       t.y += part[w].y;
     }
@@ -741,62 +769,104 @@ __device__ __forceinline__ double2 row_sum(double2 t) {
   return t;
 }
 
-// Rows of m values (S = 1): LANES threads hold a row, ITEMS packs of V values
-// each.  Threads are numbered in units of a warp, or of the block where a row
-// takes it; a unit works on group u % G of samples chunk * rows ...
-template <typename T, int V, int LANES, int ITEMS, bool BWD>
-__global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormArgs<T> p, int act) {
+// A group's S * m values in the registers of LANES threads, ITEMS packs of V
+// values each (a "row": with S = 1 it is contiguous, else S runs of m).
+// Threads are numbered in units of a warp, or of the block where a row takes it;
+// a unit works on group u % G of samples chunk * rows ...
+// FLAT: S is 1.  What limits it is registers: with the float64 sums of dweight and
+// dbias, above 32 bytes per thread weight and bias are read again for each row (they
+// stay in L1) and the next row is not fetched ahead.
+template <int LANES>
+constexpr int kRowThreads = LANES > kThreads ? LANES : kThreads;
+
+template <typename T, int V, int LANES, int ITEMS, bool BWD, bool FLAT>
+__global__ void __launch_bounds__(kRowThreads<LANES>, LANES <= kThreads && BWD && V * ITEMS * sizeof(T) <= 64 ? 2 : 1)
+    norm_rows_kernel(const NormArgs<T> p, int act) {
   constexpr int UNIT = LANES < 32 ? 32 : LANES, SUBS = UNIT / LANES;
-  const int64_t unit = (int64_t)blockIdx.x * (kThreads / UNIT) + threadIdx.x / UNIT;
+  constexpr bool KEEP = !BWD || V * ITEMS * sizeof(T) <= 32, AHEAD = KEEP;
+  const int64_t unit = (int64_t)blockIdx.x * (kRowThreads<LANES> / UNIT) + threadIdx.x / UNIT;
   if (unit >= p.G * p.chunks) return;  // whole units only
   const int64_t g = unit % p.G, chunk = unit / p.G;
   const int lane = threadIdx.x % LANES, sub = threadIdx.x % UNIT / LANES;
-  const int64_t n0 = chunk * p.rows, n1 = min(p.N, n0 + p.rows);
-  T w[ITEMS][V], b[ITEMS][V];
+  const int64_t n0 = chunk * p.rows, n1 = min(p.N, n0 + p.rows), sample = p.S * p.C;
+  // Of each pack's first value: the channel within the group, and the distance
+  // from the group's first value (below 2^31).
+  const int packs = (int)(p.m / V);  // in a run
   bool on[ITEMS];
-  double dw[BWD ? ITEMS : 1][V], db[BWD ? ITEMS : 1][V];
+  int channel[ITEMS], place[ITEMS];
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    const int64_t c = (int64_t)(k * LANES + lane) * V;
-    on[k] = c < p.m;
+    const int q = k * LANES + lane, s = FLAT ? 0 : q / packs;
+    on[k] = FLAT ? q < packs : s < (int)p.S;
+    channel[k] = (q - s * packs) * V;
+    place[k] = FLAT ? q * V : s * (int)p.C + channel[k];
+  }
+  // weight and bias of pack k
+  auto affine = [&](int k, T* w, T* b) {
+    Pack<T, V> q;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[k][i] = on[k] && p.weight ? __ldg(p.weight + g * p.m + c + i) : T(1);
-      b[k][i] = on[k] && p.bias ? __ldg(p.bias + g * p.m + c + i) : T(0);
-      if constexpr (BWD) dw[k][i] = db[k][i] = 0.0;
+    for (int i = 0; i < V; ++i) w[i] = T(1), b[i] = T(0);
+    if (!on[k]) return;
+    if (p.weight) {
+      q = load_pack<T, V>(p.weight + g * p.m + channel[k]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) w[i] = q.v[i];
     }
+    if (p.bias) {
+      q = load_pack<T, V>(p.bias + g * p.m + channel[k]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) b[i] = q.v[i];
+    }
+  };
+  T kept_w[KEEP ? ITEMS : 1][V], kept_b[KEEP ? ITEMS : 1][V];
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) affine(k, kept_w[k], kept_b[k]);
+  }
+  double dw[BWD ? ITEMS : 1][V], db[BWD ? ITEMS : 1][V];
+  if constexpr (BWD) {
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.0;
   }
   auto fetch = [&](const T* from, int64_t n, Pack<T, V>* to) {
+    from += n * sample + g * p.m;
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
       to[k] = Pack<T, V>{};
-      if (on[k] && n < n1) to[k] = load_pack<T, V>(from + n * p.C + g * p.m + (k * LANES + lane) * V);
+      if (on[k] && n < n1) to[k] = load_pack<T, V>(from + place[k]);
     }
   };
-  const double count = (double)p.m;
-  Pack<T, V> x[ITEMS], e[BWD ? ITEMS : 1], x1[ITEMS], e1[BWD ? ITEMS : 1];
+  const double count = (double)p.S * (double)p.m;
+  Pack<T, V> x[ITEMS], e[BWD ? ITEMS : 1], x1[AHEAD ? ITEMS : 1], e1[BWD && AHEAD ? ITEMS : 1];
   T mean1 = T(0), rstd1 = T(0);
-  auto fetch_next = [&](int64_t n) {
-    fetch(p.x, n, x1);
+  auto fetch_row = [&](int64_t n, Pack<T, V>* to, Pack<T, V>* to_e) {
+    fetch(p.x, n, to);
     if constexpr (BWD) {
-      fetch(p.dy, n, e1);
+      fetch(p.dy, n, to_e);
       if (n < n1) {
         mean1 = __ldg(p.mean + n * p.G + g);
         rstd1 = __ldg(p.rstd + n * p.G + g);
       }
     }
   };
-  fetch_next(n0 + sub);
+  if constexpr (AHEAD) fetch_row(n0 + sub, x1, e1);
   // Every part of a unit makes the same number of turns: row_sum is theirs together.
   for (int64_t n = n0 + sub, turns = (n1 - n0 + SUBS - 1) / SUBS; turns > 0; --turns, n += SUBS) {
+    if constexpr (AHEAD) {
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-      x[k] = x1[k];
-      if constexpr (BWD) e[k] = e1[k];
+      for (int k = 0; k < ITEMS; ++k) {
+        x[k] = x1[k];
+        if constexpr (BWD) e[k] = e1[k];
+      }
+    } else {
+      fetch_row(n, x, e);
     }
     const T mean = mean1, rstd = rstd1;
-    if (turns > 1) fetch_next(n + SUBS);
-    const int64_t at = n * p.C + g * p.m;
+    if constexpr (AHEAD)
+      if (turns > 1) fetch_row(n + SUBS, x1, e1);
+    T* const out = p.out + n * sample + g * p.m;
     if constexpr (!BWD) {
       double2 t = make_double2(0.0, 0.0);
 #pragma unroll
@@ -804,18 +874,24 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormArgs<T> p
 #pragma unroll
         for (int i = 0; i < V; ++i) t.x += (double)x[k].v[i];
       const double mu = row_sum<LANES>(t).x / count;
-      // The mean in two parts: x - high is exact near the mean.
+      // The mean in two parts: x - high is exact near the mean.  The squares go pair
+      // by pair in T and then in float64.
       const T high = (T)mu, low = (T)(mu - (double)high);
       t.x = 0.0;
 #pragma unroll
-      for (int k = 0; k < ITEMS; ++k)
+      for (int k = 0; k < ITEMS; ++k) {
+        T q[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           x[k].v[i] = (x[k].v[i] - high) - low;
-          if (on[k]) t.x = fma((double)x[k].v[i], (double)x[k].v[i], t.x);
+          q[i] = i % 2 ? fma(x[k].v[i], x[k].v[i], q[i - i % 2]) : x[k].v[i] * x[k].v[i];
         }
-      const double r64 = 1.0 / sqrt(row_sum<LANES>(t).x / count + p.eps);
-      const T r = (T)r64;
+        if (on[k]) {
+#pragma unroll
+          for (int i = V > 1 ? 1 : 0; i < V; i += 2) t.x += (double)q[i];
+        }
+      }
+      const T r = (T)(1.0 / sqrt(row_sum<LANES>(t).x / count + p.eps));
       if (n < n1) {
         if (lane == 0) {
           if (p.mean) p.mean[n * p.G + g] = (T)mu;
@@ -826,39 +902,53 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormArgs<T> p
           if (!on[k]) continue;
           Pack<T, V> o;
 #pragma unroll
-          for (int i = 0; i < V; ++i) o.v[i] = activate(act, fma(x[k].v[i] * r, w[k][i], b[k][i]));
-          store_pack<T, V>(p.out + at + (k * LANES + lane) * V, o);
+          for (int i = 0; i < V; ++i) o.v[i] = activate(act, fma(x[k].v[i] * r, kept_w[k][i], kept_b[k][i]));
+          store_pack<T, V>(out + place[k], o);
         }
       }
     } else {
-      // x becomes xhat, e becomes w dz.
+      // x becomes x - mean, e becomes w dz.  The row's sums go pair by pair in T and
+      // then in float64 (see ChannelSums).
       double2 t = make_double2(0.0, 0.0);
 #pragma unroll
       for (int k = 0; k < ITEMS; ++k) {
-        if (!on[k] || n >= n1) continue;
+        T w[V], b[V];
+        if constexpr (KEEP) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const T xh = (x[k].v[i] - mean) * rstd;
-          const T dz = e[k].v[i] * slope(act, fma(xh, w[k][i], b[k][i]));
-          const T prod = dz * xh;
-          db[k][i] += (double)dz;
-          dw[k][i] += (double)prod;
-          t.x = fma((double)w[k][i], (double)dz, t.x);
-          t.y = fma((double)w[k][i], (double)prod, t.y);
-          x[k].v[i] = xh;
-          e[k].v[i] = dz;
+          for (int i = 0; i < V; ++i) w[i] = kept_w[k][i], b[i] = kept_b[k][i];
+        } else {
+          affine(k, w, b);
+        }
+#pragma unroll
+        for (int i = 0; i < V; i += V > 1 ? 2 : 1) {
+          T z = T(0), q = T(0);
+#pragma unroll
+          for (int j = i; j < i + (V > 1 ? 2 : 1); ++j) {
+            T d = x[k].v[j] - mean, dz = e[k].v[j] * slope(act, fma(d * rstd, w[j], b[j]));
+            if (!on[k] || n >= n1) d = dz = T(0);
+            const T product = dz * (d * rstd);
+            db[k][j] += (double)dz;
+            dw[k][j] += (double)product;
+            x[k].v[j] = d;
+            e[k].v[j] = w[j] * dz;
+            z += e[k].v[j];
+            q = fma(w[j], product, q);
+          }
+          t.x += (double)z;
+          t.y += (double)q;
         }
       }
       t = row_sum<LANES>(t);
-      const T m1 = (T)(t.x / count), m2 = (T)(t.y / count);
+      // dx = rstd (w dz - m1 - xhat m2), xhat = d rstd.
+      const T m1 = (T)(t.x / count), m2 = (T)(t.y / count * (double)rstd);
       if (n < n1) {
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k) {
           if (!on[k]) continue;
           Pack<T, V> o;
 #pragma unroll
-          for (int i = 0; i < V; ++i) o.v[i] = rstd * (fma(w[k][i], e[k].v[i], -m1) - x[k].v[i] * m2);
-          store_pack<T, V>(p.out + at + (k * LANES + lane) * V, o);
+          for (int i = 0; i < V; ++i) o.v[i] = rstd * ((e[k].v[i] - m1) - x[k].v[i] * m2);
+          store_pack<T, V>(out + place[k], o);
         }
       }
     }
@@ -875,7 +965,7 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(const NormArgs<T> p
           t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
           t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
         }
-        if (on[k] && sub == 0) p.part[chunk * p.C + g * p.m + (k * LANES + lane) * V + i] = t;
+        if (on[k] && sub == 0) p.part[chunk * sample + g * p.m + place[k] + i] = t;
       }
   }
 }
@@ -924,51 +1014,62 @@ int launch_affine(Device* d, const double2* sums, int64_t rows, const NormArgs<T
   return PB_OK;
 }
 
-template <typename T, int V, int LANES, int ITEMS, bool BWD>
+template <typename T, int V, int LANES, int ITEMS, bool BWD, bool FLAT>
 int launch_rows(Device* d, int act, NormArgs<T> p) {
   constexpr int UNIT = LANES < 32 ? 32 : LANES, SUBS = UNIT / LANES;
-  const void* kernel = (const void*)norm_rows_kernel<T, V, LANES, ITEMS, BWD>;
-  // One wave of units, each at least one row per part (backward: 16, so that
-  // the sums it writes are little beside what it reads).
-  const int64_t wave = resident_blocks(d, kernel, kThreads) * (kThreads / UNIT);
+  const void* kernel = (const void*)norm_rows_kernel<T, V, LANES, ITEMS, BWD, FLAT>;
+  // One wave of units.  Backward, each has 16 rows per part at least, so that the
+  // sums it writes are little beside what it reads; two where the card were idle else.
+  const int64_t wave = resident_blocks(d, kernel, kRowThreads<LANES>) * (kRowThreads<LANES> / UNIT);
   int64_t chunks = ceil_div(wave, p.G);
   const bool sums = BWD && (p.dweight || p.dbias);
-  const int64_t most = ceil_div(p.N, (int64_t)SUBS * (sums ? 16 : 1));
+  int64_t most = ceil_div(p.N, (int64_t)SUBS * (sums ? 16 : 1));
+  if (sums && most * p.G < wave) most = ceil_div(p.N, (int64_t)SUBS * 2);
   if (chunks > most) chunks = most;
   p.rows = ceil_div(p.N, chunks);
   p.chunks = ceil_div(p.N, p.rows);
   p.part = nullptr;
   if (sums) {
     size_t bytes;
-    const int64_t e[] = {p.chunks, p.C};
-    if (!array_bytes(e, 2, sizeof(double2), &bytes)) PB_FAIL(PB_ERR_INVALID, "extents too large");
+    const int64_t e[] = {p.chunks, p.S, p.C};
+    if (!array_bytes(e, 3, sizeof(double2), &bytes)) PB_FAIL(PB_ERR_INVALID, "extents too large");
     void* ws;
     PB_CHECK(scratch(d, bytes, &ws));
     p.part = static_cast<double2*>(ws);
   }
-  const int64_t blocks = ceil_div(p.G * p.chunks, (int64_t)(kThreads / UNIT));
+  const int64_t blocks = ceil_div(p.G * p.chunks, (int64_t)(kRowThreads<LANES> / UNIT));
   if (blocks > INT32_MAX) PB_FAIL(PB_ERR_UNSUPPORTED, "too many groups");
   PB_CHECK(kt_begin(d));
-  norm_rows_kernel<T, V, LANES, ITEMS, BWD><<<(unsigned)blocks, kThreads, 0, d->stream>>>(p, act);
+  norm_rows_kernel<T, V, LANES, ITEMS, BWD, FLAT><<<(unsigned)blocks, kRowThreads<LANES>, 0, d->stream>>>(p, act);
   PB_LAUNCHED(d);
   PB_CHECK(kt_end(d));
-  return sums ? launch_affine<T>(d, p.part, p.chunks, p) : PB_OK;
+  return sums ? launch_affine<T>(d, p.part, p.chunks * p.S, p) : PB_OK;
 }
 
-// Whether rows of m values fit the rows kernel: 1024 packs at most.
-constexpr int64_t kRowPacks = 1024;
+// Packs of a row that fit the rows kernel.
+constexpr int64_t kRowPacks = 2048;
 
 template <typename T, int V, bool BWD>
 int launch_rows_of(Device* d, int act, const NormArgs<T>& p) {
-  const int64_t packs = ceil_div(p.m, (int64_t)V);
-  if (packs <= 8) return launch_rows<T, V, 8, 1, BWD>(d, act, p);
-  if (packs <= 16) return launch_rows<T, V, 8, 2, BWD>(d, act, p);
-  if (packs <= 32) return launch_rows<T, V, 16, 2, BWD>(d, act, p);
-  if (packs <= 64) return launch_rows<T, V, 32, 2, BWD>(d, act, p);
-  if (packs <= 128) return launch_rows<T, V, 32, 4, BWD>(d, act, p);
-  if (packs <= 256) return launch_rows<T, V, 256, 1, BWD>(d, act, p);
-  if (packs <= 512) return launch_rows<T, V, 256, 2, BWD>(d, act, p);
-  return launch_rows<T, V, 256, 4, BWD>(d, act, p);
+  const int64_t packs = p.S * (p.m / V);
+  if (p.S > 1) {
+    if (packs <= 8) return launch_rows<T, V, 8, 1, BWD, false>(d, act, p);
+    if (packs <= 64) return launch_rows<T, V, 32, 2, BWD, false>(d, act, p);
+    if (packs <= 256) return launch_rows<T, V, 256, 1, BWD, false>(d, act, p);
+    if (packs <= 512) return launch_rows<T, V, 256, 2, BWD, false>(d, act, p);
+    return launch_rows<T, V, 512, 4, BWD, false>(d, act, p);
+  }
+  if (packs <= 2) return launch_rows<T, V, 2, 1, BWD, true>(d, act, p);
+  if (packs <= 4) return launch_rows<T, V, 4, 1, BWD, true>(d, act, p);
+  if (packs <= 8) return launch_rows<T, V, 8, 1, BWD, true>(d, act, p);
+  if (packs <= 16) return launch_rows<T, V, 8, 2, BWD, true>(d, act, p);
+  if (packs <= 32) return launch_rows<T, V, 16, 2, BWD, true>(d, act, p);
+  if (packs <= 64) return launch_rows<T, V, 32, 2, BWD, true>(d, act, p);
+  if (packs <= 128) return launch_rows<T, V, 32, 4, BWD, true>(d, act, p);
+  if (packs <= 256) return launch_rows<T, V, 256, 1, BWD, true>(d, act, p);
+  if (packs <= 512) return launch_rows<T, V, 256, 2, BWD, true>(d, act, p);
+  if (packs <= 1024) return launch_rows<T, V, 256, 4, BWD, true>(d, act, p);
+  return launch_rows<T, V, 512, 4, BWD, true>(d, act, p);
 }
 
 // Scratch, counters and flags of the samples kernels for p.N * p.chunks units and
@@ -1061,9 +1162,9 @@ template <typename T, int V, int ACT, bool BWD>
 int launch(Device* d, const NormArgs<T>& p) {
   const int64_t lanes = ceil_div(p.C, (int64_t)V);
   const int tx = (int)(lanes < kThreads ? lanes : kThreads), ty = kThreads / tx;
-  // The ring takes rows of whole 16-byte pieces (V > 1), and at most kThreads of them.
+  // The ring takes rows of whole 16-byte pieces (V > 1), one per thread at most.
   if constexpr (V > 1)
-    if (lanes <= kThreads) return launch_ring<T, V, ACT, BWD>(d, p);
+    if (lanes <= kRingThreads) return launch_ring<T, V, ACT, BWD>(d, p);
   return launch_items<T, V, ACT, BWD>(d, p, tx, ty);
 }
 
@@ -1101,10 +1202,12 @@ int dispatch(Device* d, int act, int64_t N, int64_t S, int64_t C, int64_t G, dou
   p.m = C / G;
   p.eps = eps;
   constexpr int V = Vec16<T>::n;
-  const bool wide = C % V == 0 && (((uintptr_t)q.x | (uintptr_t)q.dy | (uintptr_t)q.out) & 15) == 0;
-  if (S == 1 && p.m <= kRowPacks * (wide && p.m % V == 0 ? V : 1))
-    return wide && p.m % V == 0 ? launch_rows_of<T, V, BWD>(d, act, p) : launch_rows_of<T, 1, BWD>(d, act, p);
-  return wide ? launch_act<T, V, BWD>(d, act, p) : launch_act<T, 1, BWD>(d, act, p);
+  const bool aligned = (((uintptr_t)q.x | (uintptr_t)q.dy | (uintptr_t)q.out | (uintptr_t)q.weight | (uintptr_t)q.bias) & 15) == 0;
+  // A group that fits the registers of a block is read once.
+  const bool packed = aligned && p.m % V == 0;
+  if (S <= kRowPacks && S * C < (int64_t(1) << 31) && S * (p.m / (packed ? V : 1)) <= kRowPacks)
+    return packed ? launch_rows_of<T, V, BWD>(d, act, p) : launch_rows_of<T, 1, BWD>(d, act, p);
+  return aligned && C % V == 0 ? launch_act<T, V, BWD>(d, act, p) : launch_act<T, 1, BWD>(d, act, p);
 }
 
 // Checks common to both directions; the bytes of x and of one sample's statistics.
