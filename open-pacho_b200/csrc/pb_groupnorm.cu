@@ -140,7 +140,8 @@ struct ChannelSums {
     *dz = dy * slope<T, ACT>(fma(d, rw[i], b[i]));
     *product = *dz * d;
   }
-  __device__ __forceinline__ void add(const Pack<T, V>& x, const Pack<T, V>& dy) {
+  // Backward, dy becomes dz.
+  __device__ __forceinline__ void add(const Pack<T, V>& x, Pack<T, V>& dy) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       if constexpr (BWD) {
@@ -148,6 +149,7 @@ struct ChannelSums {
         term(i, x.v[i], dy.v[i], &dz, &product);
         s1[i] += (double)dz;
         s2[i] += (double)product;
+        dy.v[i] = dz;
       } else {
         const double v = (double)x.v[i] - k[i];
         s1[i] += v;
@@ -155,8 +157,7 @@ struct ChannelSums {
       }
     }
   }
-  __device__ __forceinline__ void add2(const Pack<T, V>& x0, const Pack<T, V>& dy0, const Pack<T, V>& x1,
-                                       const Pack<T, V>& dy1) {
+  __device__ __forceinline__ void add2(const Pack<T, V>& x0, Pack<T, V>& dy0, const Pack<T, V>& x1, Pack<T, V>& dy1) {
     if constexpr (BWD) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -165,6 +166,8 @@ struct ChannelSums {
         term(i, x1.v[i], dy1.v[i], &z1, &q1);
         s1[i] += (double)(z0 + z1);
         s2[i] += (double)(q0 + q1);
+        dy0.v[i] = z0;
+        dy1.v[i] = z1;
       }
     } else {
       add(x0, dy0);
@@ -187,26 +190,44 @@ struct ChannelResults {
   T r1[V];                 // backward: -rstd m1; forward: the mean's low part, so that its rounding does not show
   T r2[BWD ? V : 1];       // -rstd^2 m2
 
-  // The statistics of sample n, at `stats` or in p.group.
-  __device__ __forceinline__ void begin(const NormArgs<T>& p, int64_t n, int64_t c, bool on, const double2* stats) {
+  // What does not depend on the sums of sample n; backward rw is rstd until `end`.
+  __device__ __forceinline__ void begin(const NormArgs<T>& p, int64_t n, int64_t c, bool on) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      r1[i] = on && p.weight ? __ldg(p.weight + c + i) : T(1);
+      b[i] = on && p.bias ? __ldg(p.bias + c + i) : T(0);
+      if constexpr (BWD) {
+        const int64_t g = on ? fdiv(c + i, p.by_m) : 0;
+        mean[i] = __ldg(p.mean + n * p.G + g);
+        rw[i] = __ldg(p.rstd + n * p.G + g);
+      }
+    }
+  }
+  // The statistics, at `stats` or in p.group.
+  __device__ __forceinline__ void end(const NormArgs<T>& p, int64_t n, int64_t c, bool on, const double2* stats) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int64_t g = on ? fdiv(c + i, p.by_m) : 0;
       const double2 t = stats ? stats[g] : __ldcg(p.group + n * p.G + g);
-      const T w = on && p.weight ? __ldg(p.weight + c + i) : T(1);
-      b[i] = on && p.bias ? __ldg(p.bias + c + i) : T(0);
+      const double w = (double)r1[i];
       if constexpr (BWD) {
-        mean[i] = __ldg(p.mean + n * p.G + g);
-        const double r = (double)__ldg(p.rstd + n * p.G + g);
-        rw[i] = (T)(r * (double)w);
+        const double r = (double)rw[i];
+        rw[i] = (T)(r * w);
         r1[i] = (T)(-r * t.x);
         r2[i] = (T)(-r * r * t.y);
       } else {
         mean[i] = (T)t.x;
         r1[i] = (T)(t.x - (double)mean[i]);
-        rw[i] = (T)(t.y * (double)w);
+        rw[i] = (T)(t.y * w);
       }
     }
+  }
+  // dx where dz is known.
+  __device__ __forceinline__ Pack<T, V> of_dz(const Pack<T, V>& x, const Pack<T, V>& dz) const {
+    Pack<T, V> o;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o.v[i] = fma(rw[i], dz.v[i], fma(x.v[i] - mean[i], r2[BWD ? i : 0], r1[i]));
+    return o;
   }
   __device__ __forceinline__ Pack<T, V> of(const Pack<T, V>& x, const Pack<T, V>& dy) const {
     Pack<T, V> o;
@@ -370,7 +391,8 @@ __device__ __forceinline__ void apply_item(const NormArgs<T>& p, int64_t unit, i
   const int64_t r0 = chunk * p.rows, r1 = min(p.S, r0 + p.rows);
   for (int64_t c = (int64_t)lx * V; c < p.C && ly < ty; c += (int64_t)tx * V) {
     ChannelResults<T, V, ACT, BWD> results;
-    results.begin(p, n, c, true, nullptr);
+    results.begin(p, n, c, true);
+    results.end(p, n, c, true, nullptr);
     int64_t at = (n * p.S + r0 + ly) * p.C + c;
 #pragma unroll 4
     for (int64_t r = r0 + ly; r < r1; r += ty, at += ty * p.C) {
@@ -542,18 +564,19 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
   const int c = lx * V;
   const bool on = ly < ty;
   // Stage k of the run, as copied in turn t: `two` takes two of its positions,
-  // `one` the last of an odd number.
-  auto take = [&](unsigned t, int k, int64_t n, bool wait, bool release, auto&& two, auto&& one) {
+  // `one` the last of an odd number.  With `keep` the dy that they have changed (to
+  // dz) goes back to the stage.
+  auto take = [&](unsigned t, int k, int64_t n, bool wait, bool keep, bool release, auto&& two, auto&& one) {
     const int s = t % kRing;
     if (wait) barrier_wait(full + s, (t / kRing) & 1, &failed, p.err);
-    const T* const from = ring + (size_t)s * kArrays * array + c;
+    T* const from = ring + (size_t)s * kArrays * array + c;
     const int64_t r = r0 + (int64_t)k * stage_rows;
     const int rows = on ? (int)min((int64_t)stage_rows, r1 - r) : 0;
     const int64_t at = (n * p.S + r) * p.C + c;
     int q = ly;
     for (; q + ty < rows; q += 2 * ty) {
-      const T* const f0 = from + q * C;
-      const T* const f1 = f0 + ty * C;
+      T* const f0 = from + q * C;
+      T* const f1 = f0 + ty * C;
       const Pack<T, V> x0 = *reinterpret_cast<const Pack<T, V>*>(f0), x1 = *reinterpret_cast<const Pack<T, V>*>(f1);
       Pack<T, V> d0, d1;
       if constexpr (BWD) {
@@ -561,20 +584,28 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
         d1 = *reinterpret_cast<const Pack<T, V>*>(f1 + array);
       }
       two(x0, d0, x1, d1, at + q * C, at + (q + ty) * C);
+      if (BWD && keep) {
+        *reinterpret_cast<Pack<T, V>*>(f0 + array) = d0;
+        *reinterpret_cast<Pack<T, V>*>(f1 + array) = d1;
+      }
     }
     if (q < rows) {
-      const T* const f0 = from + q * C;
+      T* const f0 = from + q * C;
       const Pack<T, V> x0 = *reinterpret_cast<const Pack<T, V>*>(f0);
       Pack<T, V> d0;
       if constexpr (BWD) d0 = *reinterpret_cast<const Pack<T, V>*>(f0 + array);
       one(x0, d0, at + q * C);
+      if (BWD && keep) *reinterpret_cast<Pack<T, V>*>(f0 + array) = d0;
     }
     if (release) {
+      // Behind this thread's own writes to the stage comes a copy of the other kind.
+      if (BWD && !wait) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if ((threadIdx.x & 31) == 0) barrier_arrive(empty + s);
     }
   };
   using P = const Pack<T, V>&;
+  using D = Pack<T, V>&;
   const bool own = p.chunks * G <= kOwnSums && G <= kOwnGroups;
   const int lanes = tx * V;                                          // channels that the threads cover, C or a little more
   const int parts = lanes < kRingThreads ? kRingThreads / lanes : 1;  // threads per channel in the sums over rows
@@ -584,9 +615,9 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
       ChannelSums<T, V, ACT, BWD> sums;
       sums.begin(p, n, c, on);
       for (int k = 0; k < stages; ++k)
-        take(turn + k, k, n, true, k < stages - held,
-             [&](P x0, P d0, P x1, P d1, int64_t, int64_t) { sums.add2(x0, d0, x1, d1); },
-             [&](P x, P dy, int64_t) { sums.add(x, dy); });
+        take(turn + k, k, n, true, k >= stages - held, k < stages - held,
+             [&](P x0, D d0, P x1, D d1, int64_t, int64_t) { sums.add2(x0, d0, x1, d1); },
+             [&](P x, D dy, int64_t) { sums.add(x, dy); });
       sums.end();
       // Over the rows of threads: red is [ty][tx * V], `parts` threads per channel.
       if (on) {
@@ -659,6 +690,8 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
         if ((threadIdx.x & 31) == 0) __stcg(p.part + unit * G + g, t);
       }
     }
+    ChannelResults<T, V, ACT, BWD> results;
+    results.begin(p, n, c, on);
     // Over the blocks of the sample.
     if (p.chunks > 1) arrive_and_wait(p.arrivals + n, (unsigned)p.chunks, p.err);
     else ring_sync();
@@ -700,15 +733,21 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
         ring_sync();
       }
     }
-    ChannelResults<T, V, ACT, BWD> results;
-    results.begin(p, n, c, on, own ? stats : nullptr);
-    auto two = [&](P x0, P d0, P x1, P d1, int64_t a0, int64_t a1) {
-      store_pack<T, V>(p.out + a0, results.of(x0, d0));
-      store_pack<T, V>(p.out + a1, results.of(x1, d1));
-    };
-    auto one = [&](P x, P dy, int64_t a) { store_pack<T, V>(p.out + a, results.of(x, dy)); };
-    for (int k = stages - held; k < stages; ++k) take(turn + k, k, n, false, true, two, one);
-    for (int k = 0; k < stages - held; ++k) take(turn + stages + k, k, n, true, true, two, one);
+    results.end(p, n, c, on, own ? stats : nullptr);
+    for (int k = stages - held; k < stages; ++k)
+      take(turn + k, k, n, false, false, true,
+           [&](P x0, P d0, P x1, P d1, int64_t a0, int64_t a1) {
+             store_pack<T, V>(p.out + a0, BWD ? results.of_dz(x0, d0) : results.of(x0, d0));
+             store_pack<T, V>(p.out + a1, BWD ? results.of_dz(x1, d1) : results.of(x1, d1));
+           },
+           [&](P x, P dz, int64_t a) { store_pack<T, V>(p.out + a, BWD ? results.of_dz(x, dz) : results.of(x, dz)); });
+    for (int k = 0; k < stages - held; ++k)
+      take(turn + stages + k, k, n, true, false, true,
+           [&](P x0, P d0, P x1, P d1, int64_t a0, int64_t a1) {
+             store_pack<T, V>(p.out + a0, results.of(x0, d0));
+             store_pack<T, V>(p.out + a1, results.of(x1, d1));
+           },
+           [&](P x, P dy, int64_t a) { store_pack<T, V>(p.out + a, results.of(x, dy)); });
     turn += 2 * stages - held;
   }
   // The last block to finish leaves the counters at zero.
@@ -780,7 +819,7 @@ template <int LANES>
 constexpr int kRowThreads = LANES > kThreads ? LANES : kThreads;
 
 template <typename T, int V, int LANES, int ITEMS, bool BWD, bool FLAT>
-__global__ void __launch_bounds__(kRowThreads<LANES>, LANES <= kThreads && BWD && V * ITEMS * sizeof(T) <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(kRowThreads<LANES>, LANES > kThreads || V * ITEMS * sizeof(T) > 64 ? 1 : BWD || V * ITEMS * sizeof(T) > 32 ? 2 : 3)
     norm_rows_kernel(const NormArgs<T> p, int act) {
   constexpr int UNIT = LANES < 32 ? 32 : LANES, SUBS = UNIT / LANES;
   constexpr bool KEEP = !BWD || V * ITEMS * sizeof(T) <= 32, AHEAD = KEEP;
@@ -1055,6 +1094,7 @@ int launch_rows_of(Device* d, int act, const NormArgs<T>& p) {
   if (p.S > 1) {
     if (packs <= 8) return launch_rows<T, V, 8, 1, BWD, false>(d, act, p);
     if (packs <= 64) return launch_rows<T, V, 32, 2, BWD, false>(d, act, p);
+    if (packs <= 128) return launch_rows<T, V, 32, 4, BWD, false>(d, act, p);
     if (packs <= 256) return launch_rows<T, V, 256, 1, BWD, false>(d, act, p);
     if (packs <= 512) return launch_rows<T, V, 256, 2, BWD, false>(d, act, p);
     return launch_rows<T, V, 512, 4, BWD, false>(d, act, p);

@@ -34,10 +34,12 @@ _FLOATS = {np.dtype(np.float32): _lib.PB_F32, np.dtype(np.float64): _lib.PB_F64}
 
 def _context(x, what):
     """(backend, dtype, dtype code) of a call's first operand."""
-    backend = getattr(getattr(x, "_data", None), "backend", None)
+    try:
+        backend, dtype = x._data.backend, x.dtype
+    except AttributeError:
+        backend = None
     if not isinstance(backend, B200Backend):
         raise TypeError(f"{what} takes arrays of the b200 backend, not {type(x).__name__}")
-    dtype = x.dtype
     code = _FLOATS.get(dtype)
     if code is None:
         raise _exc.UnsupportedDtypeError(f"{what} requires float32 or float64, not {dtype}")
@@ -66,6 +68,9 @@ def _pointer(name, x, shape, dtype, backend):
 def _output(name, given, shape, dtype, backend, template):
     """``given`` checked, or a new array like ``template``: (array, pointer)."""
     if given is not None:
+        data = given._data
+        if data.backend is backend and given.shape == shape and given.dtype is dtype:
+            return given, data.ptr
         return given, _pointer(name, given, shape, dtype, backend)
     data = backend.empty(shape, dtype)
     return wrap_like(template, data, shape, dtype, backend), data.ptr
@@ -119,8 +124,9 @@ def linear_recurrence(a, b, *, state=None, gate="linear", axis=-2, out=None, fin
     with backend._lock:
         backend._require_open()
         h, ph = _output("out", out, shape, dtype, backend, a)
-        backend._check(backend._lib.pb_recurrence(backend._ctx, 0, code, mode, outer, length, inner,
-                                                  pa, pb, ps, ph, pf), "pb_recurrence")
+        status = backend._lib.pb_recurrence(backend._ctx, 0, code, mode, outer, length, inner, pa, pb, ps, ph, pf)
+        if status:
+            backend._check(status, "pb_recurrence")
     return h
 
 
@@ -147,9 +153,10 @@ def linear_recurrence_backward(a, b, h, dh, *, state=None, dfinal=None, gate="li
         da, pda = _output("da", da, shape, dtype, backend, a)
         db, pdb = _output("db", db, shape, dtype, backend, a)
         ds, pds = _output("dstate", ds, rest, dtype, backend, a)
-        backend._check(backend._lib.pb_recurrence_backward(backend._ctx, 0, code, mode, outer, length, inner,
-                                                           pa, pb, ph, pg, ps, pf, pda, pdb, pds),
-                       "pb_recurrence_backward")
+        status = backend._lib.pb_recurrence_backward(backend._ctx, 0, code, mode, outer, length, inner, pa, pb, ph,
+                                                     pg, ps, pf, pda, pdb, pds)
+        if status:
+            backend._check(status, "pb_recurrence_backward")
     return da, db, ds
 
 
@@ -186,8 +193,10 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
         y, py = _output("y", y, shape, dtype, backend, x)
         mean, pm = _output("mean", mean, (n, groups), dtype, backend, x)
         rstd, pr = _output("rstd", rstd, (n, groups), dtype, backend, x)
-        backend._check(backend._lib.pb_group_norm(backend._ctx, 0, code, act, n, s, c, groups, float(eps),
-                                                  px, pw, pb, py, pm, pr), "pb_group_norm")
+        status = backend._lib.pb_group_norm(backend._ctx, 0, code, act, n, s, c, groups, float(eps), px, pw, pb,
+                                            py, pm, pr)
+        if status:
+            backend._check(status, "pb_group_norm")
     return y, mean, rstd
 
 
@@ -216,9 +225,10 @@ def group_norm_backward(dy, x, groups, mean, rstd, weight=None, bias=None, *, ac
             dweight, pdw = _output("dweight", dweight, (c,), dtype, backend, x)
         if bias is not None:
             dbias, pdb = _output("dbias", dbias, (c,), dtype, backend, x)
-        backend._check(backend._lib.pb_group_norm_backward(backend._ctx, 0, code, act, n, s, c, groups, pd, px,
-                                                           pm, pr, pw, pb, pdx, pdw, pdb),
-                       "pb_group_norm_backward")
+        status = backend._lib.pb_group_norm_backward(backend._ctx, 0, code, act, n, s, c, groups, pd, px, pm, pr, pw,
+                                                     pb, pdx, pdw, pdb)
+        if status:
+            backend._check(status, "pb_group_norm_backward")
     return dx, dweight, dbias
 
 
@@ -283,9 +293,11 @@ class AdamW:
             scale = _pointer("grad_scale", grad_scale, tuple(grad_scale.shape), self._dtype, b)
         with b._lock:
             b._require_open()
-            b._check(b._lib.pb_adamw(b._ctx, 0, self._code, len(g), self._p, g, self._m, self._v, self._sizes,
-                                     self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay,
-                                     self.steps + 1, scale), "pb_adamw")
+            status = b._lib.pb_adamw(b._ctx, 0, self._code, len(g), self._p, g, self._m, self._v, self._sizes,
+                                     float(self.lr), self.betas[0], self.betas[1], self.eps,
+                                     float(self.weight_decay), self.steps + 1, scale)
+            if status:
+                b._check(status, "pb_adamw")
         self.steps += 1
 
 
