@@ -390,10 +390,11 @@ int pb_reduce(pb_ctx* ctx, int dev, int op, int in_dtype, const void* src, int n
  * state when length == 0; final may be the same memory as state, which is
  * how a stream of single steps keeps its state.  Long sequences of few
  * columns are cut into chunks whose combined steps are carried in float64;
- * the result does not depend on the order in which they run.  Gates are meant
- * to be finite: behind a NaN or an Inf in a or b of its column, h is not finite
- * as long as the recurrence written above would not be, but which of the two
- * it is may differ. */
+ * the result does not depend on the order in which they run.  Behind a NaN or
+ * an Inf in a or b of its column h is not finite as long as the recurrence
+ * written above would not be, but which of the two it is may differ.  A value
+ * that leaves the range of the type inside a chunk and that later gates bring
+ * back may be there again behind the chunk. */
 enum { PB_GATE_LINEAR = 0, PB_GATE_SIGMOID = 1 };
 int pb_recurrence(pb_ctx* ctx, int dev, int dtype, int gate, int64_t outer, int64_t length,
                   int64_t inner, const void* a, const void* b, const void* state, void* h,

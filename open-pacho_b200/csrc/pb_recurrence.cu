@@ -174,13 +174,27 @@ __global__ void __launch_bounds__(kThreads) recurrence_columns_kernel(const Scan
   if (p.last) p.last[col] = BWD ? c * x : x;
 }
 
-// x -> P x + H.  0 maps to H even where P has overflowed.
-__device__ __forceinline__ double apply(const double2& map, double x) {
-  return x == 0.0 ? map.y : fma(map.x, x, map.y);
+// Maps x -> P x + H.  A product of finite factors that overflows is +-Inf, and a zero
+// wins over it: a value of 0, or a gate of 0 (a reset).  A factor that is not
+// finite makes P NaN, over which nothing wins.
+__device__ __forceinline__ bool bounded(double P) { return fabs(P) <= 1.7976931348623157e308; }
+// P v + H
+__device__ __forceinline__ double apply(double P, double v, double H) {
+  if (bounded(P)) return fma(P, v, H);
+  return v == 0.0 && isinf(P) ? H : fma(P, v, H);
 }
+// P c
+__device__ __forceinline__ double extend(double P, double c) {
+  const double q = P * c;
+  if (bounded(q)) return q;
+  if (!isfinite(c)) return c - c;
+  return c == 0.0 && isinf(P) ? 0.0 : q;
+}
+__device__ __forceinline__ double apply(const double2& map, double x) { return apply(map.x, x, map.y); }
 // The map of `a` followed by `b`.
 __device__ __forceinline__ double2 compose(const double2& a, const double2& b) {
-  return make_double2(a.x * b.x, apply(b, a.y));
+  const double P = a.x * b.x;
+  return make_double2(P != P && (a.x == 0.0 || b.x == 0.0) && !(isnan(a.x) || isnan(b.x)) ? 0.0 : P, apply(b, a.y));
 }
 
 // Asynchronous copy of BYTES into shared memory; zeros where `there` is false
@@ -317,7 +331,6 @@ __global__ void __launch_bounds__(32) recurrence_stream_kernel(const ScanArgs<T>
     }
   }
   double P = 1.0, H = 0.0;
-  T later = T(0);  // backward maps: dh of the chain step behind the one at hand
   I e = first;
   for (int64_t k = 0; k < stages; ++k) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
@@ -326,19 +339,24 @@ __global__ void __launch_bounds__(32) recurrence_stream_kernel(const ScanArgs<T>
     const T* const q = ring + slot * kStage + lane;
     slot = slot + 1 == STAGES ? 0 : slot + 1;
     const int64_t left = n - k * kRows;
-    auto one = [&](int i) {
+    // `careful`: a product may be unbounded.
+    auto one = [&](auto careful, int i) {
+      constexpr bool CAREFUL = decltype(careful)::value;
       const T a = q[i * 32], b = q[(kRows + i) * 32];
       if constexpr (MAPS && !BWD) {
         T c1, u;
         Step<T, GATE, false>::operands(a, b, &c1, &u);
-        H = u == T(0) ? H : fma(P, (double)u, H);  // 0 stays 0 behind an overflowed product
-        P *= (double)c1;
+        H = CAREFUL ? apply(P, (double)u, H) : fma(P, (double)u, H);
+        P = CAREFUL ? extend(P, (double)c1) : P * (double)c1;
       } else if constexpr (MAPS) {
         // Walking towards the chain's start: the gate of a step is the
         // coefficient of the step behind it, which came before.
         T unused = T(0);
-        if (k * kRows + i > 0) P *= (double)Step<T, GATE, true>::gate(a, &unused);
-        H = b == T(0) ? H : fma(P, (double)b, H);
+        if (k * kRows + i > 0) {
+          const double c1 = (double)Step<T, GATE, true>::gate(a, &unused);
+          P = CAREFUL ? extend(P, c1) : P * c1;
+        }
+        H = CAREFUL ? apply(P, (double)b, H) : fma(P, (double)b, H);
       } else if constexpr (!BWD) {
         T c1, u;
         Step<T, GATE, false>::operands(a, b, &c1, &u);
@@ -358,11 +376,19 @@ __global__ void __launch_bounds__(32) recurrence_stream_kernel(const ScanArgs<T>
         e -= step;
       }
     };
+    // Once a product has left float64's range, or met a NaN, it stays there: one
+    // look at the end of a stage tells whether it has to be walked with care.
+    const double P0 = P, H0 = H;
+    bool done = false;
     if (left >= kRows) {
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) one(i);
-    } else {
-      for (int i = 0; i < left; ++i) one(i);
+      for (int i = 0; i < kRows; ++i) one(std::false_type{}, i);
+      done = !MAPS || bounded(P);
+    }
+    if (!done) {
+      P = P0;
+      H = H0;
+      for (int i = 0; i < min(left, (int64_t)kRows); ++i) one(std::true_type{}, i);
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
@@ -373,7 +399,7 @@ __global__ void __launch_bounds__(32) recurrence_stream_kernel(const ScanArgs<T>
       if (s0 > 0) {
         T unused = T(0);
         const T a = __ldg(at(p.a, (I)(element<true>(p, base, s0) + step)));
-        P *= (double)Step<T, GATE, true>::gate(a, &unused);
+        P = extend(P, (double)Step<T, GATE, true>::gate(a, &unused));
       }
     }
     p.maps[item] = make_double2(P, H);

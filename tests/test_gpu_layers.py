@@ -564,3 +564,85 @@ def test_recurrence_in_several_windows(b200, dtype):
     want, bounds = ref.recurrence_backward(a, b, got, dh, state, None, "linear", ref.U[np.dtype(dtype)])
     for name, g, w, e in zip(("da", "db", "dstate"), grads, want, bounds):
         close(g.numpy(), w, e, dtype, name)
+
+
+@pytest.mark.parametrize("shape", [(1, 20000, 64), (1, 20000, 1600), (1, 3000, 9000), (1, 60, 50000)])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_recurrence_resets_behind_growth_and_poison_behind_zeros(b200, shape, dtype):
+    """A zero gate forgets whatever follows it in the product; a gate that is not
+    finite leaves nothing finite behind it, even where all it meets is zero."""
+    _, n, c = shape
+    a, b = np.full(shape, 2.0, dtype), np.zeros(shape, dtype)
+    reset, tail = n // 2, n - 25
+    a[0, reset] = 0.0
+    a[0, tail:] = 0.5
+    b[0, tail] = 1.0
+    state = np.ones((1, c), dtype)
+    state[0, 1::2] = 0.0
+    h = pb.linear_recurrence(up(b200, a), up(b200, b), state=up(b200, state)).numpy()
+    # Powers of two: the recurrence itself in the type is exact.  A column that
+    # has grown to Inf is NaN from the reset on (0 * Inf).
+    want, x = np.empty_like(h), state.copy()
+    with np.errstate(all="ignore"):
+        for t in range(n):
+            x = a[:, t] * x + b[:, t]
+            want[:, t] = x
+    finite = np.isfinite(want)
+    assert np.array_equal(h[finite], want[finite]) and not np.isfinite(h[~finite]).any()
+    assert finite[0, :, 1::2].all() and np.array_equal(h[0, tail:, 1], (0.5 ** np.arange(25)).astype(dtype))
+    a[0] = 0.5
+    b[0] = 0.0
+    a[0, 7, 3], a[0, 7, 5] = np.nan, np.inf
+    h = pb.linear_recurrence(up(b200, a), up(b200, b)).numpy()
+    assert not np.isfinite(h[0, 7:, [3, 5]]).any() and np.array_equal(np.delete(h[0], [3, 5], 1), np.zeros((n, c - 2)))
+
+
+# ---------------------------------------------------- offsets beyond 32 bits
+
+
+@pytest.mark.parametrize("steps,width", [(8200, 131072), (16400, 65600), (262500, 4100)])
+def test_recurrence_beyond_4_gib(b200, steps, width):
+    """Arrays above 4 GiB on the three ways a chain is walked: constant gates, whose
+    sums are known."""
+    torch = pytest.importorskip("torch")
+    a = torch.full((1, steps, width), 0.5, device="cuda")
+    b = torch.empty_like(a)
+    b.copy_(torch.arange(width, device="cuda", dtype=torch.float32).remainder_(7).add_(1.0))
+    h, g = torch.empty_like(a), torch.empty_like(a)
+    va, vb, vh, vg = (b200.view(t) for t in (a, b, h, g))
+    final = b200.view(torch.empty(1, width, device="cuda"))
+    pb.linear_recurrence(va, vb, out=vh, final=final)
+    # h -> 2 b; da = g h[t-1] = 2 * 2 b, db = g = 2 far from both ends.
+    pb.linear_recurrence_backward(va, None, vh, va, out=(vb, vg, final))
+    b200.synchronize()
+    want = torch.arange(width, device="cuda", dtype=torch.float32).remainder_(7).add_(1.0) * 2
+    for t in (100, steps // 2, steps - 1):
+        assert torch.allclose(h[0, t], want, rtol=1e-6), t
+    for t in (100, steps // 2, steps - 100):
+        assert torch.allclose(g[0, t], torch.ones_like(want), rtol=1e-6), t  # dh = 0.5: g = 1
+        assert torch.allclose(b[0, t], want, rtol=1e-6), t
+
+
+@pytest.mark.parametrize("shape,groups", [((2, (1 << 20) + 5, 1026), 3), ((2, 1 << 20, 1032), 8), ((1 << 21, 1, 1028), 2)])
+def test_group_norm_beyond_32_bits(b200, shape, groups):
+    """More than 2^31 values, on each kernel; the last sample against torch."""
+    torch = pytest.importorskip("torch")
+    x = torch.empty(shape, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    y = torch.empty_like(x)
+    stats = [torch.empty(shape[0], groups, device="cuda") for _ in range(2)]
+    pb.group_norm(b200.view(x), groups, activation="relu", out=tuple(b200.view(t) for t in (y, *stats)))
+    b200.synchronize()
+    last = x[-1].reshape(shape[1], groups, -1).double()
+    mean = last.mean((0, 2), keepdim=True)
+    want = ((last - mean) / (last.var((0, 2), unbiased=False, keepdim=True) + 1e-5).sqrt()).clamp(min=0)
+    assert (y[-1].reshape_as(want) - want).abs().max().item() <= 1e-5
+    del last, want
+    # dx of dy = 1 without weight and activation is 0 up to rounding.
+    x.fill_(1.0)
+    x[..., ::2] = -1.0
+    pb.group_norm(b200.view(x), groups, out=tuple(b200.view(t) for t in (y, *stats)))
+    dy = torch.ones_like(x)
+    pb.group_norm_backward(b200.view(dy), b200.view(x), groups, *(b200.view(t) for t in stats),
+                           out=(b200.view(y), None, None))
+    b200.synchronize()
+    assert y[-1].abs().max().item() <= 1e-5 and y[0].abs().max().item() <= 1e-5
