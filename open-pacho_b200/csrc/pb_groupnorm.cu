@@ -21,6 +21,8 @@
 // sums and writes the result.  Such a part of the block stays with one group and
 // walks over the samples, so that weight and bias stay in registers and the sums of
 // dweight and dbias are its own.
+#include <type_traits>
+
 #include "pb_layers.cuh"
 
 namespace pb {
@@ -764,22 +766,14 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
   }
 }
 
-template <typename T>
-__device__ __forceinline__ T activate(int act, T z) {
+// use(ACT) of the activation that a launch has.
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& use) {
   switch (act) {
-    case PB_ACT_RELU: return activate<T, PB_ACT_RELU>(z);
-    case PB_ACT_SILU: return activate<T, PB_ACT_SILU>(z);
-    case PB_ACT_GELU: return activate<T, PB_ACT_GELU>(z);
-    default: return z;
-  }
-}
-template <typename T>
-__device__ __forceinline__ T slope(int act, T z) {
-  switch (act) {
-    case PB_ACT_RELU: return slope<T, PB_ACT_RELU>(z);
-    case PB_ACT_SILU: return slope<T, PB_ACT_SILU>(z);
-    case PB_ACT_GELU: return slope<T, PB_ACT_GELU>(z);
-    default: return T(1);
+    case PB_ACT_RELU: use(std::integral_constant<int, PB_ACT_RELU>{}); break;
+    case PB_ACT_SILU: use(std::integral_constant<int, PB_ACT_SILU>{}); break;
+    case PB_ACT_GELU: use(std::integral_constant<int, PB_ACT_GELU>{}); break;
+    default: use(std::integral_constant<int, PB_ACT_NONE>{});
   }
 }
 
@@ -936,47 +930,54 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, LANES > kThreads || V * IT
           if (p.mean) p.mean[n * p.G + g] = (T)mu;
           if (p.rstd) p.rstd[n * p.G + g] = r;
         }
+        with_activation(act, [&](auto which) {
 #pragma unroll
-        for (int k = 0; k < ITEMS; ++k) {
-          if (!on[k]) continue;
-          Pack<T, V> o;
+          for (int k = 0; k < ITEMS; ++k) {
+            if (!on[k]) continue;
+            Pack<T, V> o;
 #pragma unroll
-          for (int i = 0; i < V; ++i) o.v[i] = activate(act, fma(x[k].v[i] * r, kept_w[k][i], kept_b[k][i]));
-          store_pack<T, V>(out + place[k], o);
-        }
+            for (int i = 0; i < V; ++i)
+              o.v[i] = activate<T, decltype(which)::value>(fma(x[k].v[i] * r, kept_w[k][i], kept_b[k][i]));
+            store_pack<T, V>(out + place[k], o);
+          }
+        });
       }
     } else {
       // x becomes x - mean, e becomes w dz.  The row's sums go pair by pair in T and
-      // then in float64 (see ChannelSums).
+      // then in float64 (see ChannelSums).  Packs and rows that are not there have
+      // dy = 0, and mean and rstd of 0 so that 0 times them cannot be NaN.
       double2 t = make_double2(0.0, 0.0);
+      with_activation(act, [&](auto which) {
 #pragma unroll
-      for (int k = 0; k < ITEMS; ++k) {
-        T w[V], b[V];
-        if constexpr (KEEP) {
+        for (int k = 0; k < ITEMS; ++k) {
+          const bool there = on[k] && n < n1;
+          const T mu = there ? mean : T(0), r = there ? rstd : T(0);
+          T w[V], b[V];
+          if constexpr (KEEP) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) w[i] = kept_w[k][i], b[i] = kept_b[k][i];
-        } else {
-          affine(k, w, b);
-        }
-#pragma unroll
-        for (int i = 0; i < V; i += V > 1 ? 2 : 1) {
-          T z = T(0), q = T(0);
-#pragma unroll
-          for (int j = i; j < i + (V > 1 ? 2 : 1); ++j) {
-            T d = x[k].v[j] - mean, dz = e[k].v[j] * slope(act, fma(d * rstd, w[j], b[j]));
-            if (!on[k] || n >= n1) d = dz = T(0);
-            const T product = dz * (d * rstd);
-            db[k][j] += (double)dz;
-            dw[k][j] += (double)product;
-            x[k].v[j] = d;
-            e[k].v[j] = w[j] * dz;
-            z += e[k].v[j];
-            q = fma(w[j], product, q);
+            for (int i = 0; i < V; ++i) w[i] = kept_w[k][i], b[i] = kept_b[k][i];
+          } else {
+            affine(k, w, b);
           }
-          t.x += (double)z;
-          t.y += (double)q;
+#pragma unroll
+          for (int i = 0; i < V; i += V > 1 ? 2 : 1) {
+            T z = T(0), q = T(0);
+#pragma unroll
+            for (int j = i; j < i + (V > 1 ? 2 : 1); ++j) {
+              const T d = x[k].v[j] - mu, xh = d * r;
+              const T dz = e[k].v[j] * slope<T, decltype(which)::value>(fma(xh, w[j], b[j])), product = dz * xh;
+              db[k][j] += (double)dz;
+              dw[k][j] += (double)product;
+              x[k].v[j] = d;
+              e[k].v[j] = w[j] * dz;
+              z = j == i ? e[k].v[j] : z + e[k].v[j];
+              q = j == i ? w[j] * product : fma(w[j], product, q);
+            }
+            t.x += (double)z;
+            t.y += (double)q;
+          }
         }
-      }
+      });
       t = row_sum<LANES>(t);
       // dx = rstd (w dz - m1 - xhat m2), xhat = d rstd.
       const T m1 = (T)(t.x / count), m2 = (T)(t.y / count * (double)rstd);

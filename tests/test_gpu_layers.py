@@ -262,6 +262,24 @@ def test_group_norm_far_from_zero(b200, shape, offset):
         close(q.numpy(), v, e, np.float32, name)
 
 
+@pytest.mark.parametrize("shape", [(5, 1, 100, 4), (7, 1, 96, 3), (3, 1, 5000, 1), (9, 1, 1030, 2), (17, 3, 1300, 26),
+                                   (2, 4096, 20, 4), (3, 1517, 90, 9), (1, 20000, 16, 2)])
+def test_group_norm_backward_where_the_mean_over_the_deviation_overflows(b200, shape):
+    """x = mean = 1e30 and rstd = 1e10: xhat is 0 and every gradient finite,
+    though (0 - mean) rstd, what a place without a value would give, is not.
+    Sums of 2^20 equal float32 values are exact in float64."""
+    _, w, b, rng = _norm_inputs(shape, np.float32)
+    n, s, c, g = shape
+    x, mean = np.full((n, s, c), 1e30, np.float32), np.full((n, g), 1e30, np.float32)
+    rstd, dy = np.full((n, g), 1e10, np.float32), rng.standard_normal(x.shape).astype(np.float32)
+    for act in ACTS:
+        got = pb.group_norm_backward(*(up(b200, v) for v in (dy, x)), g, *(up(b200, v) for v in (mean, rstd, w, b)),
+                                     activation=act)
+        want, bounds = ref.group_norm_backward(dy, x, g, mean, rstd, w, b, act, 2.0 ** -24)
+        for name, q, v, e in zip(("dx", "dweight", "dbias"), got, want, bounds):
+            close(q.numpy(), v, e, np.float32, f"{act} {name}")
+
+
 @pytest.mark.parametrize("shape", [(4, 1, 64, 2), (3, 700, 8, 2)])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("where", [0, 5])
