@@ -856,12 +856,23 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, LANES > kThreads || V * IT
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) affine(k, kept_w[k], kept_b[k]);
   }
-  double dw[BWD ? ITEMS : 1][V], db[BWD ? ITEMS : 1][V];
+  // In float32 the sums of dweight and dbias go FEW rows at a time in T and then in
+  // float64, which lie in shared memory, each thread's own: to convert and add every
+  // value took more of the special-function unit than the activation, and the
+  // registers of the next row.
+  constexpr bool APART = BWD && KEEP && sizeof(T) == 4 && kRowThreads<LANES> * V * ITEMS <= 2048;
+  constexpr int FEW = 4;
+  using Sum = std::conditional_t<APART, T, double>;
+  Sum dw[BWD ? ITEMS : 1][V], db[BWD ? ITEMS : 1][V];
+  __shared__ double2 whole[APART ? ITEMS * V : 1][APART ? kRowThreads<LANES> : 1];
   if constexpr (BWD) {
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.0;
+      for (int i = 0; i < V; ++i) {
+        dw[k][i] = db[k][i] = Sum(0);
+        if constexpr (APART) whole[k * V + i][threadIdx.x] = make_double2(0.0, 0.0);
+      }
   }
   auto fetch = [&](const T* from, int64_t n, Pack<T, V>* to) {
     from += n * sample + g * p.m;
@@ -966,8 +977,8 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, LANES > kThreads || V * IT
             for (int j = i; j < i + (V > 1 ? 2 : 1); ++j) {
               const T d = x[k].v[j] - mu, xh = d * r;
               const T dz = e[k].v[j] * slope<T, decltype(which)::value>(fma(xh, w[j], b[j])), product = dz * xh;
-              db[k][j] += (double)dz;
-              dw[k][j] += (double)product;
+              db[k][j] += (Sum)dz;
+              dw[k][j] += (Sum)product;
               x[k].v[j] = d;
               e[k].v[j] = w[j] * dz;
               z = j == i ? e[k].v[j] : z + e[k].v[j];
@@ -978,6 +989,18 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, LANES > kThreads || V * IT
           }
         }
       });
+      if constexpr (APART) {
+        if (turns % FEW == 1) {  // the last turn among them
+#pragma unroll
+          for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              double2& sum = whole[k * V + i][threadIdx.x];
+              sum = make_double2(sum.x + (double)db[k][i], sum.y + (double)dw[k][i]);
+              db[k][i] = dw[k][i] = Sum(0);
+            }
+        }
+      }
       t = row_sum<LANES>(t);
       // dx = rstd (w dz - m1 - xhat m2), xhat = d rstd.
       const T m1 = (T)(t.x / count), m2 = (T)(t.y / count * (double)rstd);
@@ -999,7 +1022,8 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, LANES > kThreads || V * IT
     for (int k = 0; k < ITEMS; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        double2 t = make_double2(db[k][i], dw[k][i]);
+        double2 t = make_double2((double)db[k][i], (double)dw[k][i]);
+        if constexpr (APART) t = whole[k * V + i][threadIdx.x];
 #pragma unroll
         for (int o = LANES; o < UNIT; o <<= 1) {
           t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
