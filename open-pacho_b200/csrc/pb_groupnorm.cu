@@ -29,7 +29,6 @@ namespace pb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 
 template <typename T>
 struct NormArgs {
@@ -804,16 +803,26 @@ __device__ __forceinline__ double2 row_sum(double2 t) {
 
 // A group's S * m values in the registers of LANES threads, ITEMS packs of V
 // values each (a "row": with S = 1 it is contiguous, else S runs of m).
-// Threads are numbered in units of a warp, or of the block where a row takes it;
-// a unit works on group u % G of samples chunk * rows ...
-// FLAT: S is 1.  What limits it is registers: with the float64 sums of dweight and
-// dbias, above 32 bytes per thread weight and bias are read again for each row (they
-// stay in L1) and the next row is not fetched ahead.
+// Threads are numbered in units of a warp, or of a block of LANES where a row takes
+// more than a warp; a unit works on group u % G of samples chunk * rows ...
+// FLAT: S is 1.  What limits it is registers: backward, above 32 bytes of a row per
+// thread weight and bias are read again for each row (they stay in L1) and the next
+// row is not fetched ahead.
+//
+// 16384 x 2048 in 16 groups, float32, silu, backward: 85 us, 4.7 TB/s or 73 % of the
+// copy rate, with issue slots 61 %, the special-function unit 45 % and 24 % of the
+// warps; forward 32768 x 2048 113 us, 74 %; a layer norm of 65536 x 1024 99 us, 84 %.
 template <int LANES>
-constexpr int kRowThreads = LANES > kThreads ? LANES : kThreads;
+constexpr int kRowThreads = LANES > 32 ? LANES : kThreads;
+template <int BYTES, int LANES, bool BWD>  // BYTES of a row in each thread
+constexpr int kRowBlocks = (BYTES > 64 ? 256 : BWD || BYTES > 32 ? 512 : 768) / kRowThreads<LANES> > 1
+                               ? (BYTES > 64 ? 256 : BWD || BYTES > 32 ? 512 : 768) / kRowThreads<LANES>
+                               : 1;
+template <typename T, int V, int LANES, int ITEMS, bool BWD>
+constexpr bool kRowApart = BWD && V * ITEMS * sizeof(T) <= 32 && sizeof(T) == 4;
 
 template <typename T, int V, int LANES, int ITEMS, bool BWD, bool FLAT>
-__global__ void __launch_bounds__(kRowThreads<LANES>, LANES > kThreads || V * ITEMS * sizeof(T) > 64 ? 1 : BWD || V * ITEMS * sizeof(T) > 32 ? 2 : 3)
+__global__ void __launch_bounds__(kRowThreads<LANES>, kRowBlocks<V * ITEMS * sizeof(T), LANES, BWD>)
     norm_rows_kernel(const NormArgs<T> p, int act) {
   constexpr int UNIT = LANES < 32 ? 32 : LANES, SUBS = UNIT / LANES;
   constexpr bool KEEP = !BWD || V * ITEMS * sizeof(T) <= 32, AHEAD = KEEP;
@@ -860,18 +869,19 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, LANES > kThreads || V * IT
   // float64, which lie in shared memory, each thread's own: to convert and add every
   // value took more of the special-function unit than the activation, and the
   // registers of the next row.
-  constexpr bool APART = BWD && KEEP && sizeof(T) == 4 && kRowThreads<LANES> * V * ITEMS <= 2048;
+  constexpr bool APART = kRowApart<T, V, LANES, ITEMS, BWD>;
   constexpr int FEW = 4;
   using Sum = std::conditional_t<APART, T, double>;
   Sum dw[BWD ? ITEMS : 1][V], db[BWD ? ITEMS : 1][V];
-  __shared__ double2 whole[APART ? ITEMS * V : 1][APART ? kRowThreads<LANES> : 1];
+  extern __shared__ double2 whole[];  // [ITEMS * V][kRowThreads]
+  auto apart = [&](int k, int i) -> double2& { return whole[(k * V + i) * kRowThreads<LANES> + threadIdx.x]; };
   if constexpr (BWD) {
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         dw[k][i] = db[k][i] = Sum(0);
-        if constexpr (APART) whole[k * V + i][threadIdx.x] = make_double2(0.0, 0.0);
+        if constexpr (APART) apart(k, i) = make_double2(0.0, 0.0);
       }
   }
   auto fetch = [&](const T* from, int64_t n, Pack<T, V>* to) {
@@ -995,7 +1005,7 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, LANES > kThreads || V * IT
           for (int k = 0; k < ITEMS; ++k)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-              double2& sum = whole[k * V + i][threadIdx.x];
+              double2& sum = apart(k, i);
               sum = make_double2(sum.x + (double)db[k][i], sum.y + (double)dw[k][i]);
               db[k][i] = dw[k][i] = Sum(0);
             }
@@ -1023,7 +1033,7 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, LANES > kThreads || V * IT
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         double2 t = make_double2((double)db[k][i], (double)dw[k][i]);
-        if constexpr (APART) t = whole[k * V + i][threadIdx.x];
+        if constexpr (APART) t = apart(k, i);
 #pragma unroll
         for (int o = LANES; o < UNIT; o <<= 1) {
           t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
@@ -1084,7 +1094,9 @@ int launch_rows(Device* d, int act, NormArgs<T> p) {
   const void* kernel = (const void*)norm_rows_kernel<T, V, LANES, ITEMS, BWD, FLAT>;
   // One wave of units.  Backward, each has 16 rows per part at least, so that the
   // sums it writes are little beside what it reads; two where the card were idle else.
-  const int64_t wave = resident_blocks(d, kernel, kRowThreads<LANES>) * (kRowThreads<LANES> / UNIT);
+  const size_t smem = kRowApart<T, V, LANES, ITEMS, BWD> ? sizeof(double2) * V * ITEMS * kRowThreads<LANES> : 0;
+  if (smem > 48 * 1024) PB_CHECK(allow_smem(d, kernel, smem));
+  const int64_t wave = resident_blocks(d, kernel, kRowThreads<LANES>, smem) * (kRowThreads<LANES> / UNIT);
   int64_t chunks = ceil_div(wave, p.G);
   const bool sums = BWD && (p.dweight || p.dbias);
   int64_t most = ceil_div(p.N, (int64_t)SUBS * (sums ? 16 : 1));
@@ -1104,7 +1116,7 @@ int launch_rows(Device* d, int act, NormArgs<T> p) {
   const int64_t blocks = ceil_div(p.G * p.chunks, (int64_t)(kRowThreads<LANES> / UNIT));
   if (blocks > INT32_MAX) PB_FAIL(PB_ERR_UNSUPPORTED, "too many groups");
   PB_CHECK(kt_begin(d));
-  norm_rows_kernel<T, V, LANES, ITEMS, BWD, FLAT><<<(unsigned)blocks, kRowThreads<LANES>, 0, d->stream>>>(p, act);
+  norm_rows_kernel<T, V, LANES, ITEMS, BWD, FLAT><<<(unsigned)blocks, kRowThreads<LANES>, smem, d->stream>>>(p, act);
   PB_LAUNCHED(d);
   PB_CHECK(kt_end(d));
   return sums ? launch_affine<T>(d, p.part, p.chunks * p.S, p) : PB_OK;
@@ -1113,16 +1125,27 @@ int launch_rows(Device* d, int act, NormArgs<T> p) {
 // Packs of a row that fit the rows kernel.
 constexpr int64_t kRowPacks = 2048;
 
+// Of 65 packs on.  Backward, two packs of 16 bytes are what a thread holds beside
+// the sums of their channels (16384 x 4 groups of 512: four 134 us, two 85 us); four
+// single values hold no more than one pack does (125 of them: two 149 us, four 111
+// us).  Forward, four cost a barrier less often (8192 x 4096: two 83 us, four 52 us).
+template <typename T, int V, bool BWD, bool FLAT>
+int launch_wide_rows(Device* d, int act, const NormArgs<T>& p, int64_t packs) {
+  constexpr bool TWO = BWD && V * sizeof(T) == 16;
+  if (packs <= 128) return launch_rows<T, V, TWO ? 64 : 32, TWO ? 2 : 4, BWD, FLAT>(d, act, p);
+  if (packs <= 256) return launch_rows<T, V, 128, 2, BWD, FLAT>(d, act, p);
+  if (packs <= 512) return launch_rows<T, V, 256, 2, BWD, FLAT>(d, act, p);
+  if (packs <= 1024) return launch_rows<T, V, TWO ? 512 : 256, TWO ? 2 : 4, BWD, FLAT>(d, act, p);
+  return launch_rows<T, V, 512, 4, BWD, FLAT>(d, act, p);
+}
+
 template <typename T, int V, bool BWD>
 int launch_rows_of(Device* d, int act, const NormArgs<T>& p) {
   const int64_t packs = p.S * (p.m / V);
   if (p.S > 1) {
     if (packs <= 8) return launch_rows<T, V, 8, 1, BWD, false>(d, act, p);
     if (packs <= 64) return launch_rows<T, V, 32, 2, BWD, false>(d, act, p);
-    if (packs <= 128) return launch_rows<T, V, 32, 4, BWD, false>(d, act, p);
-    if (packs <= 256) return launch_rows<T, V, 256, 1, BWD, false>(d, act, p);
-    if (packs <= 512) return launch_rows<T, V, 256, 2, BWD, false>(d, act, p);
-    return launch_rows<T, V, 512, 4, BWD, false>(d, act, p);
+    return launch_wide_rows<T, V, BWD, false>(d, act, p, packs);
   }
   if (packs <= 2) return launch_rows<T, V, 2, 1, BWD, true>(d, act, p);
   if (packs <= 4) return launch_rows<T, V, 4, 1, BWD, true>(d, act, p);
@@ -1130,11 +1153,7 @@ int launch_rows_of(Device* d, int act, const NormArgs<T>& p) {
   if (packs <= 16) return launch_rows<T, V, 8, 2, BWD, true>(d, act, p);
   if (packs <= 32) return launch_rows<T, V, 16, 2, BWD, true>(d, act, p);
   if (packs <= 64) return launch_rows<T, V, 32, 2, BWD, true>(d, act, p);
-  if (packs <= 128) return launch_rows<T, V, 32, 4, BWD, true>(d, act, p);
-  if (packs <= 256) return launch_rows<T, V, 256, 1, BWD, true>(d, act, p);
-  if (packs <= 512) return launch_rows<T, V, 256, 2, BWD, true>(d, act, p);
-  if (packs <= 1024) return launch_rows<T, V, 256, 4, BWD, true>(d, act, p);
-  return launch_rows<T, V, 512, 4, BWD, true>(d, act, p);
+  return launch_wide_rows<T, V, BWD, true>(d, act, p, packs);
 }
 
 // Scratch, counters and flags of the samples kernels for p.N * p.chunks units and

@@ -41,9 +41,6 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& r) {
   }
 }
 
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
-__device__ __forceinline__ double exp_of(double x) { return exp(x); }
-
 // 2^x and 1/x of the special-function unit: within 2 ulp and 1 ulp, results and
 // operands below 2^-126 as zero.
 __device__ __forceinline__ float exp2_unit(float x) {

@@ -202,7 +202,8 @@ NORMS = [  # (N, S, C, G)
     (1, 1, 1, 1), (1, 1, 8, 1), (32, 1, 2048, 16), (7, 1, 96, 3), (5, 1, 100, 4), (300, 1, 24, 3), (2, 1, 7, 7),
     (3, 1, 5000, 1), (2, 1, 12289, 1), (9, 1, 1030, 2), (1000, 1, 64, 1), (130, 1, 512, 2), (3, 5, 6, 2),
     (2, 49, 32, 8), (1, 1000, 3, 1), (3, 37 * 41, 90, 9), (2, 4096, 20, 4), (4, 256, 320, 32), (1, 20000, 16, 2),
-    (17, 3, 1300, 26), (600, 4, 8, 1),
+    (17, 3, 1300, 26), (600, 4, 8, 1), (20, 1, 4000, 1), (70, 1, 1000, 2), (50, 1, 1024, 1), (6, 64, 160, 4),
+    (33, 10, 64, 2),
 ]
 ACTS = [None, "relu", "silu", "gelu"]
 
