@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes as C
 from math import prod
+from operator import index
 
 import numpy as np
 
@@ -54,7 +55,7 @@ def _pointer(name, x, shape, dtype, backend):
     data = x._data
     # The usual case in three comparisons: a call's time on the host is what its
     # smallest sizes take.
-    if data.backend is backend and x.shape == shape and (x.dtype is dtype or x.dtype == dtype):
+    if data.backend is backend and x.shape == shape and (x.dtype is dtype or x.dtype == dtype) and data.ptr:
         return data.ptr
     if data.backend is not backend:
         raise _exc.BackendMismatchError(f"{name} belongs to another backend")
@@ -62,6 +63,9 @@ def _pointer(name, x, shape, dtype, backend):
         raise ValueError(f"{name} has shape {tuple(x.shape)}, expected {shape}")
     if x.dtype != dtype:
         raise ValueError(f"{name} has dtype {x.dtype}, expected {dtype}")
+    # To the C entries a null pointer is an operand that is not there.
+    if not data.ptr and prod(shape):
+        raise ValueError(f"the memory of {name} has been released")
     return data.ptr
 
 
@@ -69,7 +73,7 @@ def _output(name, given, shape, dtype, backend, template):
     """``given`` checked, or a new array like ``template``: (array, pointer)."""
     if given is not None:
         data = given._data
-        if data.backend is backend and given.shape == shape and given.dtype is dtype:
+        if data.backend is backend and given.shape == shape and given.dtype is dtype and data.ptr:
             return given, data.ptr
         return given, _pointer(name, given, shape, dtype, backend)
     data = backend.empty(shape, dtype)
@@ -165,7 +169,7 @@ def _norm_view(x, groups, what):
     shape = tuple(x.shape)
     if len(shape) < 2:
         raise ValueError(f"{what} takes (N, ..., C) arrays, channels last")
-    groups = int(groups)
+    groups = index(groups)
     if groups < 1 or shape[-1] % groups:
         raise ValueError(f"{what}: {shape[-1]} channels do not divide into {groups} groups")
     return shape[0], shape[1] if len(shape) == 3 else prod(shape[1:-1]), shape[-1], groups
@@ -239,8 +243,8 @@ class AdamW:
     The two moments are arrays of the parameters' dtype: new zeros, or the
     lists given as ``exp_avg`` and ``exp_avg_sq`` (to resume; with ``steps`` the
     number of steps already taken).  ``lr`` and ``weight_decay`` may be changed
-    between steps.  The parameters' memory must stay the same: a parameter is
-    changed in place, not replaced."""
+    between steps.  The parameters' and moments' memory must stay the same: a step
+    after one of them was released or replaced is refused."""
 
     def __init__(self, params, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
                  exp_avg=None, exp_avg_sq=None, steps=0):
@@ -255,10 +259,11 @@ class AdamW:
         self.steps = int(steps)
         self._shapes = [tuple(p.shape) for p in self.params]
         self._pointers = C.c_void_p * len(self.params)
-        self._p = self._table("params", self.params)
+        p = self._table("params", self.params)
         self.exp_avg = self._moment("exp_avg", exp_avg)
         self.exp_avg_sq = self._moment("exp_avg_sq", exp_avg_sq)
-        self._m, self._v = self._table("exp_avg", self.exp_avg), self._table("exp_avg_sq", self.exp_avg_sq)
+        self._tables = p, self._table("exp_avg", self.exp_avg), self._table("exp_avg_sq", self.exp_avg_sq)
+        self._known = [list(t) for t in self._tables]
         self._sizes = (C.c_int64 * len(self.params))(*[prod(s) for s in self._shapes])
 
     def _moment(self, name, given):
@@ -274,7 +279,7 @@ class AdamW:
             raise ValueError(f"{name}: {len(arrays)} arrays for {len(self._shapes)} parameters")
         b, dtype = self._backend, self._dtype
         pointers = [x._data.ptr for x, s in zip(arrays, self._shapes)
-                    if x._data.backend is b and x.dtype is dtype and x.shape == s]
+                    if x._data.backend is b and x.dtype is dtype and x.shape == s and x._data.ptr]
         if len(pointers) != len(arrays):  # one is not quite so: checked one by one
             pointers = [_pointer(name, x, s, dtype, b) for x, s in zip(arrays, self._shapes)]
         return self._pointers(*pointers)
@@ -285,6 +290,10 @@ class AdamW:
         multiplies every gradient (a clipping coefficient, the inverse of a
         loss scale) without a copy to the host."""
         b = self._backend
+        for arrays, known in zip((self.params, self.exp_avg, self.exp_avg_sq), self._known):
+            if [x._data.ptr or None for x in arrays] != known:
+                raise ValueError("the memory of a parameter or moment has been released or replaced")
+        p, m, v = self._tables
         g = self._table("grads", grads)
         scale = None
         if grad_scale is not None:
@@ -293,7 +302,7 @@ class AdamW:
             scale = _pointer("grad_scale", grad_scale, tuple(grad_scale.shape), self._dtype, b)
         with b._lock:
             b._require_open()
-            status = b._lib.pb_adamw(b._ctx, 0, self._code, len(g), self._p, g, self._m, self._v, self._sizes,
+            status = b._lib.pb_adamw(b._ctx, 0, self._code, len(g), p, g, m, v, self._sizes,
                                      float(self.lr), self.betas[0], self.betas[1], self.eps,
                                      float(self.weight_decay), self.steps + 1, scale)
             if status:

@@ -121,6 +121,56 @@ def test_a_closed_backend_is_refused(backend):
             call()
 
 
+def _released(backend, *shape):
+    x = _arr(backend, *shape)
+    x._data.release()
+    return x
+
+
+@pytest.mark.parametrize("call", [
+    lambda b, a: pb.linear_recurrence(a, a, state=_released(b, 2, 4)),
+    lambda b, a: pb.linear_recurrence(a, a, final=_released(b, 2, 4)),
+    lambda b, a: pb.linear_recurrence(a, a, out=_released(b, 2, 3, 4)),
+    lambda b, a: pb.linear_recurrence_backward(a, _released(b, 2, 3, 4), a, a),
+    lambda b, a: pb.linear_recurrence_backward(a, a, a, a, dfinal=_released(b, 2, 4)),
+    lambda b, a: pb.group_norm(a, 2, _released(b, 4)),
+    lambda b, a: pb.group_norm(a, 2, None, _released(b, 4)),
+    lambda b, a: pb.group_norm(a, 2, out=(None, None, _released(b, 2, 2))),
+    lambda b, a: pb.group_norm_backward(a, a, 2, *(_arr(b, 2, 2) for _ in range(2)), _arr(b, 4),
+                                        out=(None, _released(b, 4), None)),
+    lambda b, a: pb.AdamW([a, _released(b, 3)]),
+    lambda b, a: pb.AdamW([a]).step([_released(b, 2, 3, 4)]),
+    lambda b, a: pb.AdamW([a]).step([a], grad_scale=_released(b, 1)),
+])
+def test_a_released_operand_is_not_taken_for_an_absent_one(backend, call):
+    a = _arr(backend, 2, 3, 4)
+    backend._lib.pb_free = lambda *args: 0
+    with pytest.raises(ValueError, match="released"):
+        call(backend, a)
+
+
+@pytest.mark.parametrize("which", ["params", "exp_avg", "exp_avg_sq"])
+def test_adamw_refuses_memory_that_was_released_or_replaced(backend, which):
+    backend._lib.pb_free = lambda *args: 0
+    for change in (lambda opt: getattr(opt, which)[1]._data.release(),
+                   lambda opt: getattr(opt, which).__setitem__(1, _arr(backend, 5)),
+                   lambda opt: getattr(opt, which).pop()):
+        ps = [_arr(backend, 3, 4), _arr(backend, 5), _arr(backend, 0)]
+        opt = pb.AdamW(ps)
+        gs = [_arr(backend, *p.shape) for p in ps]
+        opt.step(gs)
+        change(opt)
+        with pytest.raises(ValueError, match="released or replaced"):
+            opt.step(gs)
+        assert opt.steps == 1
+
+
+def test_group_norm_takes_whole_groups_only(backend):
+    with pytest.raises(TypeError):
+        pb.group_norm(_arr(backend, 2, 3, 4), 2.5)
+    pb.group_norm(_arr(backend, 2, 3, 4), np.int64(2))
+
+
 def test_group_norm_views_and_outputs(backend):
     x, w = _arr(backend, 3, 5, 7, 8), _arr(backend, 8)
     y, mean, rstd = pb.group_norm(x, 4, w, activation="silu", eps=1e-3)
