@@ -416,7 +416,9 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) norm_samples_kernel(con
   __shared__ double2 channels[kSharedChannels];
   __shared__ unsigned item_s, epoch_s;
   __shared__ bool last;
+  __shared__ int failed;
   if (threadIdx.x == 0) {
+    failed = 0;
     item_s = atomicAdd(p.words, 1u);
     epoch_s = load_acquire(p.words + 2) + 1;
   }
@@ -451,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) norm_samples_kernel(con
         }
       }
     } else {
-      if (threadIdx.x == 0) wait_flag(p.words + kFlagWords + n, epoch, p.err);
+      if (threadIdx.x == 0) wait_until([&] { return load_acquire(p.words + kFlagWords + n) == epoch; }, &failed, p.err);
       __syncthreads();
       apply_item<T, V, ACT, BWD>(p, unit, tx, ty);
     }
@@ -487,22 +489,12 @@ __device__ __forceinline__ void ring_sync() {
 }
 
 // Wait (the whole block) until `count` blocks have arrived at *counter.
-__device__ __forceinline__ void arrive_and_wait(unsigned* counter, unsigned count, int* err) {
+__device__ __forceinline__ void arrive_and_wait(unsigned* counter, unsigned count, volatile int* failed, int* err) {
   __threadfence();
   ring_sync();
   if (threadIdx.x == 0) {
     atomicAdd(counter, 1u);
-    if (load_acquire(counter) < count) {
-      unsigned long long t0, t;
-      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-      while (load_acquire(counter) < count) {
-        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-        if (t - t0 > kFlagWaitNs) {
-          atomicExch(err, KERR_WAIT_TIMEOUT);
-          break;
-        }
-      }
-    }
+    wait_until([&] { return load_acquire(counter) >= count; }, failed, err);
   }
   ring_sync();
 }
@@ -694,7 +686,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
     ChannelResults<T, V, ACT, BWD> results;
     results.begin(p, n, c, on);
     // Over the blocks of the sample.
-    if (p.chunks > 1) arrive_and_wait(p.arrivals + n, (unsigned)p.chunks, p.err);
+    if (p.chunks > 1) arrive_and_wait(p.arrivals + n, (unsigned)p.chunks, &failed, p.err);
     else ring_sync();
     const int wide = min(G, kRingThreads), rows = kRingThreads / wide;
     const int first = own ? 0 : (int)chunk, step = own ? 1 : (int)p.chunks;  // groups this block adds up
@@ -728,7 +720,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
       ring_sync();
     }
     if (!own) {
-      if (p.chunks > 1) arrive_and_wait(p.arrivals + n, 2 * (unsigned)p.chunks, p.err);
+      if (p.chunks > 1) arrive_and_wait(p.arrivals + n, 2 * (unsigned)p.chunks, &failed, p.err);
       else {
         __threadfence();
         ring_sync();
@@ -1321,7 +1313,7 @@ int pb_group_norm(pb_ctx* ctx, int dev, int dtype, int act, int64_t N, int64_t S
                   const void* x, const void* weight, const void* bias, void* y, void* mean, void* rstd) {
   size_t bytes, stats;
   PB_CHECK(check_view(ctx, dtype, act, N, S, C, G, &bytes, &stats));
-  if (!(eps >= 0.0)) PB_FAIL(PB_ERR_INVALID, "eps is not negative");
+  if (!(eps >= 0.0)) PB_FAIL(PB_ERR_INVALID, "eps is negative or NaN");
   if (!N) return PB_OK;
   if (!x || !y) PB_FAIL(PB_ERR_INVALID, "null operand");
   const size_t item = dtype == PB_F32 ? 4 : 8, line = (size_t)C * item;

@@ -90,7 +90,7 @@ __device__ __forceinline__ double sigmoid(double z) { return 1.0 / (1.0 + exp(-z
 // An item waits only for flags of items with lower numbers, which are running or
 // done when it gets its own, so every wait ends.
 constexpr int kFlagWords = 4;
-constexpr unsigned long long kFlagWaitNs = 4ull * 1000 * 1000 * 1000;
+constexpr unsigned long long kFlagWaitNs = 4ull * 1000 * 1000 * 1000, kShortWaitNs = 1000 * 1000;
 
 __device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
   unsigned v;
@@ -100,15 +100,19 @@ __device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
 __device__ __forceinline__ void store_release(unsigned* p, unsigned v) {
   asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
 }
-// Wait for a flag of this launch; after kFlagWaitNs the error word is set and the
-// kernel goes on to its end (with wrong values).
-__device__ __forceinline__ void wait_flag(const unsigned* flag, unsigned epoch, int* err) {
-  if (load_acquire(flag) == epoch) return;
+// Wait until reached(): after kFlagWaitNs the error word and `failed` (the block's)
+// are set and the kernel goes on to its end (with wrong values), its further waits
+// being short.
+template <typename F>
+__device__ __forceinline__ void wait_until(F&& reached, volatile int* failed, int* err) {
+  if (reached()) return;
   unsigned long long t0, t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  while (load_acquire(flag) != epoch) {
+  const unsigned long long limit = *failed ? kShortWaitNs : kFlagWaitNs;
+  while (!reached()) {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (t - t0 > kFlagWaitNs) {
+    if (t - t0 > limit) {
+      *failed = 1;
       atomicExch(err, KERR_WAIT_TIMEOUT);
       return;
     }
@@ -129,9 +133,7 @@ __device__ __forceinline__ void finish_words(unsigned* words, unsigned epoch, un
 
 // ---- runs of memory on their way into shared memory ------------------------
 //
-// Bulk copies that report to an mbarrier.  Every wait is bounded: after
-// kFlagWaitNs the error word and `failed` are set and the kernel goes on to its
-// end (with wrong values), its further waits being short.
+// Bulk copies that report to an mbarrier.  Every wait is bounded, as above.
 __device__ __forceinline__ uint32_t shared_address(const void* p) {
   return (uint32_t)__cvta_generic_to_shared(p);
 }
@@ -156,19 +158,9 @@ __device__ __forceinline__ bool barrier_try(uint64_t* bar, unsigned parity) {
   return done != 0;
 }
 __device__ __forceinline__ bool barrier_wait(uint64_t* bar, unsigned parity, volatile int* failed, int* err) {
-  if (barrier_try(bar, parity)) return true;
-  unsigned long long t0, t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  const unsigned long long limit = *failed ? 1000 * 1000 : kFlagWaitNs;
-  while (!barrier_try(bar, parity)) {
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (t - t0 > limit) {
-      *failed = 1;
-      atomicExch(err, KERR_WAIT_TIMEOUT);
-      return false;
-    }
-  }
-  return true;
+  bool done = false;
+  wait_until([&] { return done = barrier_try(bar, parity); }, failed, err);
+  return done;
 }
 // `bytes` (a multiple of 16) from global to shared memory, both 16-byte aligned.
 __device__ __forceinline__ void bulk_copy(void* to, const void* from, unsigned bytes, uint64_t* bar) {

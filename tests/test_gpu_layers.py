@@ -9,6 +9,7 @@ again from their true start (at most two roundings where one was counted)."""
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import numpy as np
 import pytest
@@ -665,3 +666,41 @@ def test_group_norm_beyond_32_bits(b200, shape, groups):
                            out=(b200.view(y), None, None))
     b200.synchronize()
     assert y[-1].abs().max().item() <= 1e-5 and y[0].abs().max().item() <= 1e-5
+
+
+def test_two_contexts_at_once(b200):
+    """Kernels whose blocks wait for one another, from two threads on two streams
+    of one GPU: each is launched whole, so neither waits for the other."""
+    shapes = [(2, 2048, 320, 32), (2, 4096, 20, 4), (3, 1517, 90, 9)]
+    backends = [pb.B200Backend(), pb.B200Backend()]
+    failed = []
+
+    def work(backend, seed):
+        try:
+            rng = np.random.default_rng(seed)
+            sets = []
+            for n, s, c, g in shapes:
+                x, dy = (up(backend, rng.standard_normal((n, s, c)).astype(np.float32)) for _ in range(2))
+                w, b = (up(backend, rng.standard_normal(c).astype(np.float32)) for _ in range(2))
+                sets.append((x, dy, g, w, b))
+            first = None
+            for _ in range(15):
+                bits = []
+                for x, dy, g, w, b in sets:
+                    y, mean, rstd = pb.group_norm(x, g, w, b, activation="silu")
+                    grads = pb.group_norm_backward(dy, x, g, mean, rstd, w, b, activation="silu")
+                    h = pb.linear_recurrence(x, dy, gate="sigmoid")
+                    bits += [v.numpy().tobytes() for v in (y, mean, rstd, h) + grads]
+                first = first or bits
+                assert bits == first
+        except BaseException as e:  # noqa: BLE001 - reported by the test's own thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(b, i)) for i, b in enumerate(backends)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for b in backends:
+        b.close()
+    assert not failed, failed[0]
