@@ -21,6 +21,7 @@ or another output, except ``final`` with ``state``.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 from math import prod
 from operator import index
 
@@ -263,7 +264,7 @@ class AdamW:
         self.exp_avg = self._moment("exp_avg", exp_avg)
         self.exp_avg_sq = self._moment("exp_avg_sq", exp_avg_sq)
         self._tables = p, self._table("exp_avg", self.exp_avg), self._table("exp_avg_sq", self.exp_avg_sq)
-        self._known = [list(t) for t in self._tables]
+        self._known = [[x._data.ptr for x in q] for q in (self.params, self.exp_avg, self.exp_avg_sq)]
         self._sizes = (C.c_int64 * len(self.params))(*[prod(s) for s in self._shapes])
 
     def _moment(self, name, given):
@@ -281,8 +282,9 @@ class AdamW:
         pointers = [x._data.ptr for x, s in zip(arrays, self._shapes)
                     if x._data.backend is b and x.dtype is dtype and x.shape == s and x._data.ptr]
         if len(pointers) != len(arrays):  # one is not quite so: checked one by one
-            pointers = [_pointer(name, x, s, dtype, b) for x, s in zip(arrays, self._shapes)]
-        return self._pointers(*pointers)
+            pointers = [_pointer(name, x, s, dtype, b) or 0 for x, s in zip(arrays, self._shapes)]
+        # Through an array of integers: ctypes takes four times as long for each item.
+        return self._pointers.from_buffer(array("Q", pointers))
 
     def step(self, grads, *, grad_scale=None):
         """One step with a gradient array per parameter (shape and dtype of
@@ -291,7 +293,7 @@ class AdamW:
         loss scale) without a copy to the host."""
         b = self._backend
         for arrays, known in zip((self.params, self.exp_avg, self.exp_avg_sq), self._known):
-            if [x._data.ptr or None for x in arrays] != known:
+            if [x._data.ptr for x in arrays] != known:
                 raise ValueError("the memory of a parameter or moment has been released or replaced")
         p, m, v = self._tables
         g = self._table("grads", grads)
