@@ -110,7 +110,8 @@ __device__ __forceinline__ double shift_of(const NormArgs<T>& p, int64_t n, int6
 // Channels whose sums a block holds in shared memory.
 constexpr int64_t kSharedChannels = 1024;
 
-// What a thread needs of its V channels: the sums of one pass over positions.
+// What a thread needs of its V channels c, c + step, ...: the sums of one pass over
+// positions.  Channels from C on have sums that nobody reads.
 // Backward, xhat = rstd d with d = x - mean, so the second sum is formed of
 // dz d and takes its factor rstd at the end.  Two positions at a time: their
 // terms are added in T and the pair in float64, which halves the conversions (they
@@ -121,16 +122,18 @@ struct ChannelSums {
   double k[BWD ? 1 : V];
   T mean[BWD ? V : 1], rstd[BWD ? V : 1], rw[BWD ? V : 1], b[BWD ? V : 1];
 
-  __device__ __forceinline__ void begin(const NormArgs<T>& p, int64_t n, int64_t c, bool on) {
+  __device__ __forceinline__ void begin(const NormArgs<T>& p, int64_t n, int64_t c, bool on, int step = 1) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       s1[i] = s2[i] = 0.0;
-      const int64_t g = on ? fdiv(c + i, p.by_m) : 0;
+      const int64_t ch = c + i * step;
+      const bool here = on && ch < p.C;
+      const int64_t g = here ? fdiv(ch, p.by_m) : 0;
       if constexpr (BWD) {
         mean[i] = __ldg(p.mean + n * p.G + g);
         rstd[i] = __ldg(p.rstd + n * p.G + g);
-        rw[i] = on && p.weight ? rstd[i] * __ldg(p.weight + c + i) : rstd[i];
-        b[i] = on && p.bias ? __ldg(p.bias + c + i) : T(0);
+        rw[i] = here && p.weight ? rstd[i] * __ldg(p.weight + ch) : rstd[i];
+        b[i] = here && p.bias ? __ldg(p.bias + ch) : T(0);
       } else {
         k[i] = shift_of(p, n, g);
       }
@@ -192,23 +195,27 @@ struct ChannelResults {
   T r2[BWD ? V : 1];       // -rstd^2 m2
 
   // What does not depend on the sums of sample n; backward rw is rstd until `end`.
-  __device__ __forceinline__ void begin(const NormArgs<T>& p, int64_t n, int64_t c, bool on) {
+  __device__ __forceinline__ void begin(const NormArgs<T>& p, int64_t n, int64_t c, bool on, int step = 1) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      r1[i] = on && p.weight ? __ldg(p.weight + c + i) : T(1);
-      b[i] = on && p.bias ? __ldg(p.bias + c + i) : T(0);
+      const int64_t ch = c + i * step;
+      const bool here = on && ch < p.C;
+      r1[i] = here && p.weight ? __ldg(p.weight + ch) : T(1);
+      b[i] = here && p.bias ? __ldg(p.bias + ch) : T(0);
       if constexpr (BWD) {
-        const int64_t g = on ? fdiv(c + i, p.by_m) : 0;
+        const int64_t g = here ? fdiv(ch, p.by_m) : 0;
         mean[i] = __ldg(p.mean + n * p.G + g);
         rw[i] = __ldg(p.rstd + n * p.G + g);
       }
     }
   }
   // The statistics, at `stats` or in p.group.
-  __device__ __forceinline__ void end(const NormArgs<T>& p, int64_t n, int64_t c, bool on, const double2* stats) {
+  __device__ __forceinline__ void end(const NormArgs<T>& p, int64_t n, int64_t c, bool on, const double2* stats,
+                                      int step = 1) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int64_t g = on ? fdiv(c + i, p.by_m) : 0;
+      const int64_t ch = c + i * step;
+      const int64_t g = on && ch < p.C ? fdiv(ch, p.by_m) : 0;
       const double2 t = stats ? stats[g] : __ldcg(p.group + n * p.G + g);
       const double w = (double)r1[i];
       if constexpr (BWD) {
@@ -476,6 +483,12 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) norm_samples_kernel(con
 // and the others come from L2.  What is left besides the copies is the chain
 // between the passes (sums over the block's rows and groups, publishing,
 // waiting, adding up), about 5 us for each round of samples.
+//
+// SPREAD: rows of any size.  A stage's values start and end anywhere, its copy on
+// the 16-byte boundaries around them, the last values of the array apart; a thread's
+// channels lie tx apart, so that lanes move neighbours one value at a time.
+// 8 x 4096 x 319 float32 forward 33 us (plain loads of norm_samples_kernel: 69; 320
+// channels: 31), backward 63 (124; 54); 6 x 3001 x 1107 forward 64 (125).
 constexpr int kRingThreads = 480;  // and a warp that copies: 16 warps, 128 registers each thread
 constexpr int kRingWarps = kRingThreads / 32;
 constexpr int kRing = 8;
@@ -499,15 +512,24 @@ __device__ __forceinline__ void arrive_and_wait(unsigned* counter, unsigned coun
   ring_sync();
 }
 
-template <typename T, int V, int ACT, bool BWD>
+// Values of one array of a stage.
+template <typename T, bool SPREAD>
+__host__ __device__ __forceinline__ int64_t ring_array(int64_t stage_rows, int64_t C) {
+  constexpr int A = 16 / (int)sizeof(T);
+  return SPREAD ? (stage_rows * C + 2 * A - 2) / A * A : stage_rows * C;
+}
+
+template <typename T, int V, int ACT, bool BWD, bool SPREAD>
 __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const NormArgs<T> p, int tx, int ty,
                                                                        int stage_rows, int64_t together) {
   constexpr int kArrays = BWD ? 2 : 1;
+  constexpr int A = 16 / (int)sizeof(T);
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) uint64_t full[kRing], empty[kRing];
   __shared__ int failed;
   __shared__ bool last;
-  const int C = (int)p.C, G = (int)p.G, m = (int)p.m, array = stage_rows * C;  // values of one array of a stage
+  const int C = (int)p.C, G = (int)p.G, m = (int)p.m;
+  const int array = (int)ring_array<T, SPREAD>(stage_rows, C);
   T* const ring = reinterpret_cast<T*>(smem);
   double2* const red = reinterpret_cast<double2*>(ring + (size_t)kRing * kArrays * array);  // [V * kRingThreads]
   double2* const channels = red + V * kRingThreads;                                          // [C]
@@ -539,12 +561,27 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
         if (!ok) break;
         const int64_t r = r0 + (int64_t)(k < stages ? k : k - stages) * stage_rows;
         const int rows = (int)min((int64_t)stage_rows, r1 - r);
-        const unsigned bytes = (unsigned)(rows * C) * (unsigned)sizeof(T);
-        const int64_t at = (n * p.S + r) * p.C;
+        int64_t at = (n * p.S + r) * p.C, end = at + (int64_t)rows * C;
         T* const to = ring + (size_t)s * kArrays * array;
+        if constexpr (SPREAD) {
+          const int64_t all = p.N * p.S * p.C, stop = min((end + A - 1) & -(int64_t)A, all & -(int64_t)A);
+          at &= -(int64_t)A;
+          if (end > stop) {
+            for (int64_t e = max(stop, at); e < end; ++e) {
+              to[e - at] = __ldg(p.x + e);
+              if constexpr (BWD) to[array + (e - at)] = __ldg(p.dy + e);
+            }
+            // A later copy to this stage comes behind these writes.
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+          end = max(stop, at);
+        }
+        const unsigned bytes = (unsigned)(end - at) * (unsigned)sizeof(T);
         barrier_expect(full + s, bytes * kArrays);
-        bulk_copy(to, p.x + at, bytes, full + s);
-        if constexpr (BWD) bulk_copy(to + array, p.dy + at, bytes, full + s);
+        if (!SPREAD || bytes) {
+          bulk_copy(to, p.x + at, bytes, full + s);
+          if constexpr (BWD) bulk_copy(to + array, p.dy + at, bytes, full + s);
+        }
       }
     }
     // Nothing may be on its way when the block ends.
@@ -554,41 +591,61 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
   }
 
   const int lx = threadIdx.x % tx, ly = threadIdx.x / tx;
-  const int c = lx * V;
+  const int c = SPREAD ? lx : lx * V, apart = SPREAD ? tx : 1;  // the first channel, and how far the others are
   const bool on = ly < ty;
+  // Packs of this thread's channels in shared memory, and the result's.
+  auto get = [&](const T* from) {
+    Pack<T, V> o;
+    if constexpr (SPREAD) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) o.v[i] = from[i * tx];
+    } else {
+      o = *reinterpret_cast<const Pack<T, V>*>(from);
+    }
+    return o;
+  };
+  auto put = [&](T* to, const Pack<T, V>& o) {
+    if constexpr (SPREAD) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (c + i * tx < C) to[i * tx] = o.v[i];
+    } else {
+      *reinterpret_cast<Pack<T, V>*>(to) = o;
+    }
+  };
   // Stage k of the run, as copied in turn t: `two` takes two of its positions,
   // `one` the last of an odd number.  With `keep` the dy that they have changed (to
   // dz) goes back to the stage.
   auto take = [&](unsigned t, int k, int64_t n, bool wait, bool keep, bool release, auto&& two, auto&& one) {
     const int s = t % kRing;
     if (wait) barrier_wait(full + s, (t / kRing) & 1, &failed, p.err);
-    T* const from = ring + (size_t)s * kArrays * array + c;
     const int64_t r = r0 + (int64_t)k * stage_rows;
     const int rows = on ? (int)min((int64_t)stage_rows, r1 - r) : 0;
     const int64_t at = (n * p.S + r) * p.C + c;
+    T* const from = ring + (size_t)s * kArrays * array + c + (SPREAD ? (int)((at - c) & (A - 1)) : 0);
     int q = ly;
     for (; q + ty < rows; q += 2 * ty) {
       T* const f0 = from + q * C;
       T* const f1 = f0 + ty * C;
-      const Pack<T, V> x0 = *reinterpret_cast<const Pack<T, V>*>(f0), x1 = *reinterpret_cast<const Pack<T, V>*>(f1);
+      const Pack<T, V> x0 = get(f0), x1 = get(f1);
       Pack<T, V> d0, d1;
       if constexpr (BWD) {
-        d0 = *reinterpret_cast<const Pack<T, V>*>(f0 + array);
-        d1 = *reinterpret_cast<const Pack<T, V>*>(f1 + array);
+        d0 = get(f0 + array);
+        d1 = get(f1 + array);
       }
       two(x0, d0, x1, d1, at + q * C, at + (q + ty) * C);
       if (BWD && keep) {
-        *reinterpret_cast<Pack<T, V>*>(f0 + array) = d0;
-        *reinterpret_cast<Pack<T, V>*>(f1 + array) = d1;
+        put(f0 + array, d0);
+        put(f1 + array, d1);
       }
     }
     if (q < rows) {
       T* const f0 = from + q * C;
-      const Pack<T, V> x0 = *reinterpret_cast<const Pack<T, V>*>(f0);
+      const Pack<T, V> x0 = get(f0);
       Pack<T, V> d0;
-      if constexpr (BWD) d0 = *reinterpret_cast<const Pack<T, V>*>(f0 + array);
+      if constexpr (BWD) d0 = get(f0 + array);
       one(x0, d0, at + q * C);
-      if (BWD && keep) *reinterpret_cast<Pack<T, V>*>(f0 + array) = d0;
+      if (BWD && keep) put(f0 + array, d0);
     }
     if (release) {
       // Behind this thread's own writes to the stage comes a copy of the other kind.
@@ -597,6 +654,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
       if ((threadIdx.x & 31) == 0) barrier_arrive(empty + s);
     }
   };
+  auto store = [&](int64_t a, const Pack<T, V>& o) { put(p.out + a, o); };
   using P = const Pack<T, V>&;
   using D = Pack<T, V>&;
   const bool own = p.chunks * G <= kOwnSums && G <= kOwnGroups;
@@ -606,7 +664,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
     const int64_t unit = n * p.chunks + chunk;
     {
       ChannelSums<T, V, ACT, BWD> sums;
-      sums.begin(p, n, c, on);
+      sums.begin(p, n, c, on, apart);
       for (int k = 0; k < stages; ++k)
         take(turn + k, k, n, true, k >= stages - held, k < stages - held,
              [&](P x0, D d0, P x1, D d1, int64_t, int64_t) { sums.add2(x0, d0, x1, d1); },
@@ -642,7 +700,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
         t.x += red[k * lanes + q].x;
         t.y += red[k * lanes + q].y;
       }
-      const int ch = q % tx * V + q / tx;
+      const int ch = SPREAD ? q : q % tx * V + q / tx;
       if (ch < C) {
         if (BWD && p.chan) {
           double2* const all = p.chan + (int64_t)blockIdx.x * C + ch;  // over the block's samples
@@ -684,7 +742,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
       }
     }
     ChannelResults<T, V, ACT, BWD> results;
-    results.begin(p, n, c, on);
+    results.begin(p, n, c, on, apart);
     // Over the blocks of the sample.
     if (p.chunks > 1) arrive_and_wait(p.arrivals + n, (unsigned)p.chunks, &failed, p.err);
     else ring_sync();
@@ -726,21 +784,21 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
         ring_sync();
       }
     }
-    results.end(p, n, c, on, own ? stats : nullptr);
+    results.end(p, n, c, on, own ? stats : nullptr, apart);
     for (int k = stages - held; k < stages; ++k)
       take(turn + k, k, n, false, false, true,
            [&](P x0, P d0, P x1, P d1, int64_t a0, int64_t a1) {
-             store_pack<T, V>(p.out + a0, BWD ? results.of_dz(x0, d0) : results.of(x0, d0));
-             store_pack<T, V>(p.out + a1, BWD ? results.of_dz(x1, d1) : results.of(x1, d1));
+             store(a0, BWD ? results.of_dz(x0, d0) : results.of(x0, d0));
+             store(a1, BWD ? results.of_dz(x1, d1) : results.of(x1, d1));
            },
-           [&](P x, P dz, int64_t a) { store_pack<T, V>(p.out + a, BWD ? results.of_dz(x, dz) : results.of(x, dz)); });
+           [&](P x, P dz, int64_t a) { store(a, BWD ? results.of_dz(x, dz) : results.of(x, dz)); });
     for (int k = 0; k < stages - held; ++k)
       take(turn + stages + k, k, n, true, false, true,
            [&](P x0, P d0, P x1, P d1, int64_t a0, int64_t a1) {
-             store_pack<T, V>(p.out + a0, results.of(x0, d0));
-             store_pack<T, V>(p.out + a1, results.of(x1, d1));
+             store(a0, results.of(x0, d0));
+             store(a1, results.of(x1, d1));
            },
-           [&](P x, P dy, int64_t a) { store_pack<T, V>(p.out + a, results.of(x, dy)); });
+           [&](P x, P dy, int64_t a) { store(a, results.of(x, dy)); });
     turn += 2 * stages - held;
   }
   // The last block to finish leaves the counters at zero.
@@ -1196,7 +1254,7 @@ int launch_items(Device* d, NormArgs<T> p, int tx, int ty) {
   return BWD && (p.dweight || p.dbias) ? launch_affine<T>(d, p.chan, units, p) : PB_OK;
 }
 
-template <typename T, int V, int ACT, bool BWD>
+template <typename T, int V, int ACT, bool BWD, bool SPREAD>
 int launch_ring(Device* d, NormArgs<T> p) {
   constexpr int kArrays = BWD ? 2 : 1;
   const int tx = (int)ceil_div(p.C, (int64_t)V), ty = kRingThreads / tx;
@@ -1205,9 +1263,10 @@ int launch_ring(Device* d, NormArgs<T> p) {
   // The ring takes what is left of shared memory; positions per stage in
   // pairs per thread where they fit.
   int64_t stage_rows = ((int64_t)kRingSmem - fixed) / kRing / row_bytes;
+  if (SPREAD) stage_rows = ((int64_t)kRingSmem - fixed - kRing * kArrays * 32) / kRing / row_bytes;  // two boundaries
   if (stage_rows > 2 * ty) stage_rows = stage_rows / (2 * ty) * (2 * ty);
-  const void* kernel = (const void*)norm_ring_kernel<T, V, ACT, BWD>;
-  const size_t bytes = (size_t)(kRing * stage_rows * row_bytes + fixed);
+  const void* kernel = (const void*)norm_ring_kernel<T, V, ACT, BWD, SPREAD>;
+  const size_t bytes = (size_t)(kRing * kArrays * ring_array<T, SPREAD>(stage_rows, p.C) * (int64_t)sizeof(T) + fixed);
   PB_CHECK(allow_smem(d, kernel, kRingSmem));
   const int64_t wave = d->sm_count;
   // Samples worked on together: their operands stay in L2 between the passes,
@@ -1238,9 +1297,11 @@ template <typename T, int V, int ACT, bool BWD>
 int launch(Device* d, const NormArgs<T>& p) {
   const int64_t lanes = ceil_div(p.C, (int64_t)V);
   const int tx = (int)(lanes < kThreads ? lanes : kThreads), ty = kThreads / tx;
-  // The ring takes rows of whole 16-byte pieces (V > 1), one per thread at most.
-  if constexpr (V > 1)
-    if (lanes <= kRingThreads) return launch_ring<T, V, ACT, BWD>(d, p);
+  // The ring takes rows that its threads span, of whole 16-byte pieces (V > 1) or not.
+  constexpr bool SPREAD = V == 1;
+  constexpr int VR = Vec16<T>::n;
+  if ((((uintptr_t)p.x | (uintptr_t)p.dy) & 15) == 0 && ceil_div(p.C, (int64_t)VR) <= kRingThreads)
+    return launch_ring<T, VR, ACT, BWD, SPREAD>(d, p);
   return launch_items<T, V, ACT, BWD>(d, p, tx, ty);
 }
 

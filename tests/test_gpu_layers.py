@@ -205,6 +205,9 @@ NORMS = [  # (N, S, C, G)
     (2, 49, 32, 8), (1, 1000, 3, 1), (3, 37 * 41, 90, 9), (2, 4096, 20, 4), (4, 256, 320, 32), (1, 20000, 16, 2),
     (17, 3, 1300, 26), (600, 4, 8, 1), (20, 1, 4000, 1), (70, 1, 1000, 2), (50, 1, 1024, 1), (6, 64, 160, 4),
     (33, 10, 64, 2),
+    # Rows that do not end on 16 bytes, the ends of the array among them; wider than a block spans.
+    (1, 2049, 1, 1), (3, 5000, 21, 3), (5, 1031, 91, 7), (3, 700, 319, 11), (2, 333, 959, 7), (3, 333, 1919, 19),
+    (2, 150, 1921, 17), (2, 2050, 5, 1), (1, 40001, 7, 7),
 ]
 ACTS = [None, "relu", "silu", "gelu"]
 
@@ -321,6 +324,31 @@ def test_group_norm_without_statistics(b200):
         _lib.check(b200._lib.pb_group_norm(b200._ctx, 0, _lib.PB_F32, 0, *shape, 1e-5, dx._data.ptr, None, None,
                                            y._data.ptr, None, None))
         assert y.numpy().tobytes() == want.tobytes()
+
+
+@pytest.mark.parametrize("shape", [(2, 700, 64, 4), (3, 1, 64, 4), (2, 700, 9, 3)])
+@pytest.mark.parametrize("odd", ["x", "dy", "weight", "dx", "dweight"])
+def test_group_norm_backward_of_arrays_that_start_anywhere(b200, shape, odd):
+    """The C entry takes pointers that are aligned to a value only, and leaves
+    what lies around its results."""
+    x, w, b, rng = _norm_inputs(shape, np.float32)
+    n, s, c, g = shape
+    dy = rng.standard_normal(x.shape).astype(np.float32)
+    (_, mean, rstd), _ = ref.group_norm(x, g, w, b, 1e-3, "silu", 0.0)
+    mean, rstd = mean.astype(np.float32), rstd.astype(np.float32)
+    arrays = dict(dy=dy, x=x, mean=mean, rstd=rstd, weight=w, bias=b, dx=np.full_like(x, np.nan),
+                  dweight=np.full_like(w, np.nan), dbias=np.full_like(b, np.nan))
+    held = {k: up(b200, np.concatenate([np.full(8, 7, np.float32), v.ravel(), np.full(8, 7, np.float32)]))
+            for k, v in arrays.items()}
+    at = {k: 9 if k == odd else 8 for k in arrays}
+    held[odd] = up(b200, np.concatenate([np.full(9, 7, np.float32), arrays[odd].ravel(), np.full(7, 7, np.float32)]))
+    _lib.check(b200._lib.pb_group_norm_backward(b200._ctx, 0, _lib.PB_F32, _lib.ACTIVATIONS["silu"], *shape,
+                                                *(held[k]._data.ptr + 4 * at[k] for k in arrays)))
+    want, bounds = ref.group_norm_backward(dy, x, g, mean, rstd, w, b, "silu", 2.0 ** -24)
+    for k, v, e in zip(("dx", "dweight", "dbias"), want, bounds):
+        got = held[k].numpy()
+        close(got[at[k]:at[k] + v.size].reshape(v.shape), v, e, np.float32, k)
+        assert np.all(got[:at[k]] == 7) and np.all(got[at[k] + v.size:] == 7)
 
 
 def test_group_norm_repeats_its_bits(b200):
