@@ -826,27 +826,26 @@ __device__ __forceinline__ void with_activation(int act, F&& use) {
   }
 }
 
-// Sums of two numbers over the LANES threads that share a row, the same in
+__device__ __forceinline__ double plus(double a, double b) { return a + b; }
+__device__ __forceinline__ double2 plus(double2 a, double2 b) { return make_double2(a.x + b.x, a.y + b.y); }
+__device__ __forceinline__ double across(double t, int o) { return __shfl_xor_sync(0xffffffffu, t, o); }
+__device__ __forceinline__ double2 across(double2 t, int o) { return make_double2(across(t.x, o), across(t.y, o)); }
+
+// Sums (double or double2) over the LANES threads that share a row, the same in
 // each of them and in a fixed order.
-template <int LANES>
-__device__ __forceinline__ double2 row_sum(double2 t) {
+template <int LANES, typename S>
+__device__ __forceinline__ S row_sum(S t) {
   constexpr int kRowWarps = LANES / 32;
 #pragma unroll
-  for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) {
-    t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
-    t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
-  }
+  for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) t = plus(t, across(t, o));
   if constexpr (LANES > 32) {
-    __shared__ double2 part[kRowWarps];
+    __shared__ S part[kRowWarps];
     __syncthreads();  // the last use of `part` is over
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = t;
     __syncthreads();
     t = part[0];
 #pragma unroll
-    for (int w = 1; w < kRowWarps; ++w) {
-      t.x += part[w].x;
-      t.y += part[w].y;
-    }
+    for (int w = 1; w < kRowWarps; ++w) t = plus(t, part[w]);
   }
   return t;
 }
@@ -859,9 +858,8 @@ __device__ __forceinline__ double2 row_sum(double2 t) {
 // thread weight and bias are read again for each row (they stay in L1) and the next
 // row is not fetched ahead.
 //
-// 16384 x 2048 in 16 groups, float32, silu, backward: 85 us, 4.7 TB/s or 73 % of the
-// copy rate, with issue slots 61 %, the special-function unit 45 % and 24 % of the
-// warps; forward 32768 x 2048 113 us, 74 %; a layer norm of 65536 x 1024 99 us, 84 %.
+// 16384 x 2048 in 16 groups, float32, silu, backward: 83 us, 4.9 TB/s or 76 % of the
+// copy rate; forward 32768 x 2048 103 us, 81 %; a layer norm of 65536 x 1024 99 us, 84 %.
 template <int LANES>
 constexpr int kRowThreads = LANES > 32 ? LANES : kThreads;
 template <int BYTES, int LANES, bool BWD>  // BYTES of a row in each thread
@@ -942,7 +940,7 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, kRowBlocks<V * ITEMS * siz
       if (on[k] && n < n1) to[k] = load_pack<T, V>(from + place[k]);
     }
   };
-  const double count = (double)p.S * (double)p.m;
+  const double share = 1.0 / ((double)p.S * (double)p.m);
   Pack<T, V> x[ITEMS], e[BWD ? ITEMS : 1], x1[AHEAD ? ITEMS : 1], e1[BWD && AHEAD ? ITEMS : 1];
   T mean1 = T(0), rstd1 = T(0);
   auto fetch_row = [&](int64_t n, Pack<T, V>* to, Pack<T, V>* to_e) {
@@ -972,16 +970,16 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, kRowBlocks<V * ITEMS * siz
       if (turns > 1) fetch_row(n + SUBS, x1, e1);
     T* const out = p.out + n * sample + g * p.m;
     if constexpr (!BWD) {
-      double2 t = make_double2(0.0, 0.0);
+      double t = 0.0;
 #pragma unroll
       for (int k = 0; k < ITEMS; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) t.x += (double)x[k].v[i];
-      const double mu = row_sum<LANES>(t).x / count;
+        for (int i = 0; i < V; ++i) t += (double)x[k].v[i];
+      const double mu = row_sum<LANES>(t) * share;
       // The mean in two parts: x - high is exact near the mean.  The squares go pair
       // by pair in T and then in float64.
       const T high = (T)mu, low = (T)(mu - (double)high);
-      t.x = 0.0;
+      t = 0.0;
 #pragma unroll
       for (int k = 0; k < ITEMS; ++k) {
         T q[V];
@@ -992,10 +990,10 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, kRowBlocks<V * ITEMS * siz
         }
         if (on[k]) {
 #pragma unroll
-          for (int i = V > 1 ? 1 : 0; i < V; i += 2) t.x += (double)q[i];
+          for (int i = V > 1 ? 1 : 0; i < V; i += 2) t += (double)q[i];
         }
       }
-      const T r = (T)(1.0 / sqrt(row_sum<LANES>(t).x / count + p.eps));
+      const T r = (T)rsqrt(row_sum<LANES>(t) * share + p.eps);
       if (n < n1) {
         if (lane == 0) {
           if (p.mean) p.mean[n * p.G + g] = (T)mu;
@@ -1063,7 +1061,7 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, kRowBlocks<V * ITEMS * siz
       }
       t = row_sum<LANES>(t);
       // dx = rstd (w dz - m1 - xhat m2), xhat = d rstd.
-      const T m1 = (T)(t.x / count), m2 = (T)(t.y / count * (double)rstd);
+      const T m1 = (T)(t.x * share), m2 = (T)(t.y * share * (double)rstd);
       if (n < n1) {
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k) {
@@ -1172,21 +1170,33 @@ int launch_rows(Device* d, int act, NormArgs<T> p) {
   return sums ? launch_affine<T>(d, p.part, p.chunks * p.S, p) : PB_OK;
 }
 
-// Packs of a row that fit the rows kernel.
+// Packs of 16 bytes of a row that fit the rows kernel.
 constexpr int64_t kRowPacks = 2048;
 
 // Of 65 packs on.  Backward, two packs of 16 bytes are what a thread holds beside
-// the sums of their channels (16384 x 4 groups of 512: four 134 us, two 85 us); four
-// single values hold no more than one pack does (125 of them: two 149 us, four 111
-// us).  Forward, four cost a barrier less often (8192 x 4096: two 83 us, four 52 us).
+// the sums of their channels (16384 x 4 groups of 512: four 134 us, two 85 us).
+// Forward, four cost a barrier less often (8192 x 4096: two 83 us, four 52 us).
+// Single values (V = 1): as many as two packs hold, so that a warp does up to 256
+// (4547 x 42 groups of 169 forward: a block of 128 threads 261 us, a warp 66 us).
 template <typename T, int V, bool BWD, bool FLAT>
 int launch_wide_rows(Device* d, int act, const NormArgs<T>& p, int64_t packs) {
-  constexpr bool TWO = BWD && V * sizeof(T) == 16;
-  if (packs <= 128) return launch_rows<T, V, TWO ? 64 : 32, TWO ? 2 : 4, BWD, FLAT>(d, act, p);
-  if (packs <= 256) return launch_rows<T, V, 128, 2, BWD, FLAT>(d, act, p);
-  if (packs <= 512) return launch_rows<T, V, 256, 2, BWD, FLAT>(d, act, p);
-  if (packs <= 1024) return launch_rows<T, V, TWO ? 512 : 256, TWO ? 2 : 4, BWD, FLAT>(d, act, p);
-  return launch_rows<T, V, 512, 4, BWD, FLAT>(d, act, p);
+  constexpr bool TWO = BWD && V > 1;
+  constexpr int K = V > 1 ? 2 : 32 / (int)sizeof(T);  // 32 bytes of a row to a thread
+  if constexpr (V > 1) {
+    if (packs <= 128) return launch_rows<T, V, TWO ? 64 : 32, TWO ? 2 : 4, BWD, FLAT>(d, act, p);
+    if (packs <= 256) return launch_rows<T, V, 128, 2, BWD, FLAT>(d, act, p);
+    if (packs <= 512) return launch_rows<T, V, 256, 2, BWD, FLAT>(d, act, p);
+    if (packs <= 1024) return launch_rows<T, V, TWO ? 512 : 256, TWO ? 2 : 4, BWD, FLAT>(d, act, p);
+    return launch_rows<T, V, 512, 4, BWD, FLAT>(d, act, p);
+  } else {
+    if (packs <= 128) return launch_rows<T, V, 32, 4, BWD, FLAT>(d, act, p);
+    if (packs <= 256) return launch_rows<T, V, 256 / K, K, BWD, FLAT>(d, act, p);
+    if (packs <= 512) return launch_rows<T, V, 512 / K, K, BWD, FLAT>(d, act, p);
+    if (packs <= 1024) return launch_rows<T, V, 1024 / K, K, BWD, FLAT>(d, act, p);
+    if (packs <= 2048) return launch_rows<T, V, 2048 / K, K, BWD, FLAT>(d, act, p);
+    if (K * 512 > 2048 && packs <= K * 512) return launch_rows<T, V, 512, K, BWD, FLAT>(d, act, p);
+    return launch_rows<T, V, 512, 2 * K, BWD, FLAT>(d, act, p);
+  }
 }
 
 template <typename T, int V, bool BWD>
@@ -1200,9 +1210,15 @@ int launch_rows_of(Device* d, int act, const NormArgs<T>& p) {
   if (packs <= 2) return launch_rows<T, V, 2, 1, BWD, true>(d, act, p);
   if (packs <= 4) return launch_rows<T, V, 4, 1, BWD, true>(d, act, p);
   if (packs <= 8) return launch_rows<T, V, 8, 1, BWD, true>(d, act, p);
-  if (packs <= 16) return launch_rows<T, V, 8, 2, BWD, true>(d, act, p);
-  if (packs <= 32) return launch_rows<T, V, 16, 2, BWD, true>(d, act, p);
-  if (packs <= 64) return launch_rows<T, V, 32, 2, BWD, true>(d, act, p);
+  if constexpr (V > 1) {
+    if (packs <= 16) return launch_rows<T, V, 8, 2, BWD, true>(d, act, p);
+    if (packs <= 32) return launch_rows<T, V, 16, 2, BWD, true>(d, act, p);
+    if (packs <= 64) return launch_rows<T, V, 32, 2, BWD, true>(d, act, p);
+  } else {
+    if (packs <= 16) return launch_rows<T, V, 4, 4, BWD, true>(d, act, p);
+    if (packs <= 32) return launch_rows<T, V, 8, 4, BWD, true>(d, act, p);
+    if (packs <= 64) return launch_rows<T, V, 16, 4, BWD, true>(d, act, p);
+  }
   return launch_wide_rows<T, V, BWD, true>(d, act, p, packs);
 }
 
@@ -1342,7 +1358,7 @@ int dispatch(Device* d, int act, int64_t N, int64_t S, int64_t C, int64_t G, dou
   const bool aligned = (((uintptr_t)q.x | (uintptr_t)q.dy | (uintptr_t)q.out | (uintptr_t)q.weight | (uintptr_t)q.bias) & 15) == 0;
   // A group that fits the registers of a block is read once.
   const bool packed = aligned && p.m % V == 0;
-  if (S <= kRowPacks && S * C < (int64_t(1) << 31) && S * (p.m / (packed ? V : 1)) <= kRowPacks)
+  if (S <= kRowPacks * V && S * C < (int64_t(1) << 31) && S * p.m <= kRowPacks * V)
     return packed ? launch_rows_of<T, V, BWD>(d, act, p) : launch_rows_of<T, 1, BWD>(d, act, p);
   return aligned && C % V == 0 ? launch_act<T, V, BWD>(d, act, p) : launch_act<T, 1, BWD>(d, act, p);
 }

@@ -47,7 +47,8 @@ def close(got, want, bound, dtype, what):
 SHAPES = [  # (outer, length, inner): single steps, short, odd, long, wide, one column
     (1, 1, 1), (32, 1, 2048), (3, 2, 5), (1, 7, 33), (2, 8, 31), (5, 17, 64), (2, 127, 40), (2, 128, 32),
     (2, 129, 96), (1, 1000, 515), (3, 2047, 100), (1, 4100, 8), (1, 20011, 1), (700, 9, 1), (9, 300, 3),
-    (1, 16381, 65), (64, 40, 1024),
+    (1, 16381, 65), (64, 40, 1024), (2, 70, 33), (3, 211, 71), (5, 641, 38), (1, 333, 1), (2, 4099, 149), (300, 50, 31),
+    (1, 40, 8193), (13, 97, 701),
 ]
 
 
@@ -208,6 +209,9 @@ NORMS = [  # (N, S, C, G)
     # Rows that do not end on 16 bytes, the ends of the array among them; wider than a block spans.
     (1, 2049, 1, 1), (3, 5000, 21, 3), (5, 1031, 91, 7), (3, 700, 319, 11), (2, 333, 959, 7), (3, 333, 1919, 19),
     (2, 150, 1921, 17), (2, 2050, 5, 1), (1, 40001, 7, 7),
+    # Rows of single values, from a few lanes to the most that a block holds, and one more.
+    (40, 1, 39, 3), (60, 1, 62, 2), (30, 1, 507, 3), (20, 1, 510, 1), (9, 1, 1022, 1), (6, 1, 4095, 1), (5, 1, 8191, 1),
+    (3, 1, 8193, 1), (9, 3, 25, 1), (7, 41, 50, 2), (5, 101, 15, 1),
 ]
 ACTS = [None, "relu", "silu", "gelu"]
 
