@@ -1309,15 +1309,17 @@ int launch_ring(Device* d, NormArgs<T> p) {
   return BWD && (p.dweight || p.dbias) ? launch_affine<T>(d, p.chan, together * p.chunks, p) : PB_OK;
 }
 
+// The ring takes rows that its threads span, of whole 16-byte pieces or not.
+template <typename T>
+bool ring_takes(const NormArgs<T>& p) {
+  return (((uintptr_t)p.x | (uintptr_t)p.dy) & 15) == 0 && ceil_div(p.C, (int64_t)Vec16<T>::n) <= kRingThreads;
+}
+
 template <typename T, int V, int ACT, bool BWD>
 int launch(Device* d, const NormArgs<T>& p) {
   const int64_t lanes = ceil_div(p.C, (int64_t)V);
   const int tx = (int)(lanes < kThreads ? lanes : kThreads), ty = kThreads / tx;
-  // The ring takes rows that its threads span, of whole 16-byte pieces (V > 1) or not.
-  constexpr bool SPREAD = V == 1;
-  constexpr int VR = Vec16<T>::n;
-  if ((((uintptr_t)p.x | (uintptr_t)p.dy) & 15) == 0 && ceil_div(p.C, (int64_t)VR) <= kRingThreads)
-    return launch_ring<T, VR, ACT, BWD, SPREAD>(d, p);
+  if (ring_takes(p)) return launch_ring<T, Vec16<T>::n, ACT, BWD, V == 1>(d, p);
   return launch_items<T, V, ACT, BWD>(d, p, tx, ty);
 }
 
@@ -1356,9 +1358,12 @@ int dispatch(Device* d, int act, int64_t N, int64_t S, int64_t C, int64_t G, dou
   p.eps = eps;
   constexpr int V = Vec16<T>::n;
   const bool aligned = (((uintptr_t)q.x | (uintptr_t)q.dy | (uintptr_t)q.out | (uintptr_t)q.weight | (uintptr_t)q.bias) & 15) == 0;
-  // A group that fits the registers of a block is read once.
-  const bool packed = aligned && p.m % V == 0;
-  if (S <= kRowPacks * V && S * C < (int64_t(1) << 31) && S * p.m <= kRowPacks * V)
+  // A group that fits the registers of a block is read once.  It then gives a row of
+  // sums for dweight and dbias per position: with many positions the ring's sums of
+  // whole runs are less to add up (float32 backward, rows and ring: 16 x 64 x 1280 in 32
+  // groups 19 and 23 us, 16 x 300 x 640 in 32 42 and 27, 32 x 8000 x 8 in 8 876 and 23).
+  const bool packed = aligned && p.m % V == 0, by_rows = !BWD || S <= 64 || !(q.dweight || q.dbias) || !ring_takes(p);
+  if (by_rows && S <= kRowPacks * V && S * C < (int64_t(1) << 31) && S * p.m <= kRowPacks * V)
     return packed ? launch_rows_of<T, V, BWD>(d, act, p) : launch_rows_of<T, 1, BWD>(d, act, p);
   return aligned && C % V == 0 ? launch_act<T, V, BWD>(d, act, p) : launch_act<T, 1, BWD>(d, act, p);
 }
