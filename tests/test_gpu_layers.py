@@ -330,6 +330,22 @@ def test_group_norm_without_statistics(b200):
         assert y.numpy().tobytes() == want.tobytes()
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("shape", [(5, 1, 100, 4), (6, 64, 160, 4), (5, 101, 15, 1), (2, 333, 24, 3), (3, 2000, 8, 8),
+                                   (3, 4000, 2, 1), (2, 8000, 3, 3), (2, 5000, 21, 3), (2, 150, 1921, 17)])
+def test_group_norm_backward_without_weight_and_bias(b200, shape, dtype):
+    x, _, _, rng = _norm_inputs(shape, dtype, 2)
+    g = shape[3]
+    dy = rng.standard_normal(x.shape).astype(dtype)
+    (_, mean, rstd), _ = ref.group_norm(x, g, None, None, 1e-3, "silu", 0.0)
+    mean, rstd = mean.astype(dtype), rstd.astype(dtype)
+    dx, dw, db = pb.group_norm_backward(up(b200, dy), up(b200, x), g, up(b200, mean), up(b200, rstd),
+                                        activation="silu", out=(poisoned(b200, x.shape, dtype), None, None))
+    want, bounds = ref.group_norm_backward(dy, x, g, mean, rstd, None, None, "silu", ref.U[np.dtype(dtype)])
+    close(dx.numpy(), want[0], bounds[0], dtype, "dx")
+    assert dw is None and db is None
+
+
 @pytest.mark.parametrize("shape", [(2, 700, 64, 4), (3, 1, 64, 4), (2, 700, 9, 3)])
 @pytest.mark.parametrize("odd", ["x", "dy", "weight", "dx", "dweight"])
 def test_group_norm_backward_of_arrays_that_start_anywhere(b200, shape, odd):
