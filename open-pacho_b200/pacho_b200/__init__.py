@@ -12,7 +12,8 @@
 * :mod:`pacho_b200.distributed` -- the sharded forms (batch split, row blocks
   with B broadcast, norm and DOT partials over NVLink) for one process per GPU.
 * :mod:`pacho_b200.layers` -- :func:`linear_recurrence`, :func:`group_norm`, their
-  backward passes and :class:`AdamW`: a sequence layer and its training step.
+  backward passes, :class:`AdamW` and :func:`adamw_step`: a sequence layer and its
+  training step.
 * :func:`devices` -- the visible B200s as OpenPacho-style ``DeviceInfo``.
 * :class:`DeviceArray` -- a typed view of a device buffer, returned by this
   package's own functions when they are not handed OpenPacho arrays.
@@ -23,6 +24,7 @@ from .discovery import DeviceInfo, devices
 from .exceptions import BackendMismatchError, BackendUnavailableError, UnsupportedDtypeError
 from .layers import (
     AdamW,
+    adamw_step,
     group_norm,
     group_norm_backward,
     linear_recurrence,
@@ -41,6 +43,7 @@ __all__ = [
     "DeviceBuffer",
     "DeviceInfo",
     "UnsupportedDtypeError",
+    "adamw_step",
     "devices",
     "group_norm",
     "group_norm_backward",

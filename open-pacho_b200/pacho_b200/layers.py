@@ -5,7 +5,8 @@
   with a kept state (serving) to long sequences, and its gradients;
 * :func:`group_norm` / :func:`group_norm_backward` -- group norm with an
   activation, channels last, and its gradients (layer norm is one group);
-* :class:`AdamW` -- the optimizer step over many tensors in one call.
+* :class:`AdamW` -- the optimizer step over many tensors in one call, and
+  :func:`adamw_step`, the same on lists that the caller keeps.
 
 OpenPacho has none of these (its reductions, src/openpacho/_reductions.py, and
 its norm, src/openpacho/_norm.py, are the nearest).  Arrays are anything with
@@ -237,6 +238,64 @@ def group_norm_backward(dy, x, groups, mean, rstd, weight=None, bias=None, *, ac
     return dx, dweight, dbias
 
 
+def _table(name, arrays, shapes, dtype, backend):
+    """The host table of device pointers of one list, an array for each shape."""
+    if len(arrays) != len(shapes):
+        raise ValueError(f"{name}: {len(arrays)} arrays for {len(shapes)} parameters")
+    pointers = [x._data.ptr for x, s in zip(arrays, shapes)
+                if x._data.backend is backend and x.dtype is dtype and x.shape == s and x._data.ptr]
+    if len(pointers) != len(arrays):  # one is not quite so: checked one by one
+        pointers = [_pointer(name, x, s, dtype, backend) or 0 for x, s in zip(arrays, shapes)]
+    # Through an array of integers: ctypes takes four times as long for each item.
+    return (C.c_void_p * len(pointers)).from_buffer(array("Q", pointers))
+
+
+def _sizes(shapes):
+    return (C.c_int64 * len(shapes))(*[prod(s) for s in shapes])
+
+
+def _two(betas):
+    betas = tuple(float(v) for v in betas)
+    if len(betas) != 2:
+        raise ValueError("betas are two numbers")
+    return betas
+
+
+def _adamw(backend, dtype, code, tables, sizes, grad_scale, lr, betas, eps, weight_decay, step):
+    """One step over host tables of parameters, gradients and the two moments."""
+    scale = None
+    if grad_scale is not None:
+        if prod(grad_scale.shape) != 1:
+            raise ValueError("grad_scale has one element")
+        scale = _pointer("grad_scale", grad_scale, tuple(grad_scale.shape), dtype, backend)
+    with backend._lock:
+        backend._require_open()
+        status = backend._lib.pb_adamw(backend._ctx, 0, code, len(sizes), *tables, sizes, float(lr), *betas,
+                                       float(eps), float(weight_decay), step, scale)
+        if status:
+            backend._check(status, "pb_adamw")
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
+               weight_decay=0.01, grad_scale=None):
+    """One AdamW step with decoupled weight decay over lists of arrays, in place and
+    in one call: parameters, their gradients and the two moments, each list with
+    an array of the parameter's shape and dtype for each parameter.
+
+    ``step`` counts from 1 and is the caller's to keep; :class:`AdamW` keeps it and
+    the moments.  ``grad_scale``, a one-element array on the GPU, multiplies every
+    gradient (a clipping coefficient, the inverse of a loss scale) without a copy to
+    the host."""
+    params = list(params)
+    if not params:
+        raise ValueError("adamw_step needs at least one parameter")
+    backend, dtype, code = _context(params[0], "adamw_step")
+    shapes = [tuple(p.shape) for p in params]
+    tables = [_table(name, arrays, shapes, dtype, backend) for name, arrays in
+              (("params", params), ("grads", grads), ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq))]
+    _adamw(backend, dtype, code, tables, _sizes(shapes), grad_scale, lr, _two(betas), eps, weight_decay, index(step))
+
+
 class AdamW:
     """AdamW with decoupled weight decay over a list of parameter arrays, which
     :meth:`step` updates in place, all tensors in one call.
@@ -254,18 +313,15 @@ class AdamW:
             raise ValueError("AdamW needs at least one parameter")
         self._backend, self._dtype, self._code = _context(self.params[0], "AdamW")
         self.lr, self.eps, self.weight_decay = float(lr), float(eps), float(weight_decay)
-        self.betas = tuple(float(v) for v in betas)
-        if len(self.betas) != 2:
-            raise ValueError("betas are two numbers")
+        self.betas = _two(betas)
         self.steps = int(steps)
         self._shapes = [tuple(p.shape) for p in self.params]
-        self._pointers = C.c_void_p * len(self.params)
         p = self._table("params", self.params)
         self.exp_avg = self._moment("exp_avg", exp_avg)
         self.exp_avg_sq = self._moment("exp_avg_sq", exp_avg_sq)
         self._tables = p, self._table("exp_avg", self.exp_avg), self._table("exp_avg_sq", self.exp_avg_sq)
         self._known = [[x._data.ptr for x in q] for q in (self.params, self.exp_avg, self.exp_avg_sq)]
-        self._sizes = (C.c_int64 * len(self.params))(*[prod(s) for s in self._shapes])
+        self._sizes = _sizes(self._shapes)
 
     def _moment(self, name, given):
         if given is not None:
@@ -275,45 +331,23 @@ class AdamW:
                 for p, s in zip(self.params, self._shapes)]
 
     def _table(self, name, arrays):
-        """The host table of device pointers of one list."""
-        if len(arrays) != len(self._shapes):
-            raise ValueError(f"{name}: {len(arrays)} arrays for {len(self._shapes)} parameters")
-        b, dtype = self._backend, self._dtype
-        pointers = [x._data.ptr for x, s in zip(arrays, self._shapes)
-                    if x._data.backend is b and x.dtype is dtype and x.shape == s and x._data.ptr]
-        if len(pointers) != len(arrays):  # one is not quite so: checked one by one
-            pointers = [_pointer(name, x, s, dtype, b) or 0 for x, s in zip(arrays, self._shapes)]
-        # Through an array of integers: ctypes takes four times as long for each item.
-        return self._pointers.from_buffer(array("Q", pointers))
+        return _table(name, arrays, self._shapes, self._dtype, self._backend)
 
     def step(self, grads, *, grad_scale=None):
         """One step with a gradient array per parameter (shape and dtype of
-        the parameter).  ``grad_scale``, a one-element array on the GPU,
-        multiplies every gradient (a clipping coefficient, the inverse of a
-        loss scale) without a copy to the host."""
-        b = self._backend
+        the parameter) and ``grad_scale`` as of :func:`adamw_step`."""
         for arrays, known in zip((self.params, self.exp_avg, self.exp_avg_sq), self._known):
             if [x._data.ptr for x in arrays] != known:
                 raise ValueError("the memory of a parameter or moment has been released or replaced")
         p, m, v = self._tables
-        g = self._table("grads", grads)
-        scale = None
-        if grad_scale is not None:
-            if prod(grad_scale.shape) != 1:
-                raise ValueError("grad_scale has one element")
-            scale = _pointer("grad_scale", grad_scale, tuple(grad_scale.shape), self._dtype, b)
-        with b._lock:
-            b._require_open()
-            status = b._lib.pb_adamw(b._ctx, 0, self._code, len(g), p, g, m, v, self._sizes,
-                                     float(self.lr), self.betas[0], self.betas[1], self.eps,
-                                     float(self.weight_decay), self.steps + 1, scale)
-            if status:
-                b._check(status, "pb_adamw")
+        _adamw(self._backend, self._dtype, self._code, (p, self._table("grads", grads), m, v), self._sizes, grad_scale,
+               self.lr, self.betas, self.eps, self.weight_decay, self.steps + 1)
         self.steps += 1
 
 
 __all__ = [
     "AdamW",
+    "adamw_step",
     "group_norm",
     "group_norm_backward",
     "linear_recurrence",

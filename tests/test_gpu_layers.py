@@ -414,6 +414,25 @@ def test_adamw(b200, sizes, dtype, scale):
 
 
 @pytest.mark.parametrize("dtype", FLOATS)
+def test_adamw_step_on_the_callers_lists(b200, dtype):
+    """The optimizer's bits, from lists and a step number that the caller keeps."""
+    sizes = [3, 0, 2049, 8192]
+    a = _adamw_inputs(sizes, dtype)
+    mine, its = ({k: [up(b200, x) for x in v] for k, v in a.items()} for _ in range(2))
+    scale = up(b200, np.array([0.37], dtype))
+    opt = pb.AdamW(its["p"], lr=0.02, betas=(0.9, 0.99), eps=1e-6, weight_decay=0.1, exp_avg=its["m"],
+                   exp_avg_sq=its["v"], steps=4)
+    for step in (5, 6):
+        pb.adamw_step(mine["p"], mine["g"], mine["m"], mine["v"], step=step, lr=0.02, betas=(0.9, 0.99), eps=1e-6,
+                      weight_decay=0.1, grad_scale=scale)
+        opt.step(its["g"], grad_scale=scale)
+    for k in "pmv":
+        for x, y, old in zip(mine[k], its[k], a[k]):
+            assert x.numpy().tobytes() == y.numpy().tobytes()
+            assert not x.size or x.numpy().tobytes() != old.tobytes()
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
 def test_adamw_views_at_odd_places_leave_their_neighbours(b200, dtype):
     """Tensors inside one buffer that start anywhere (the C entry asks only for
     whole elements): what lies between them stays as it was."""

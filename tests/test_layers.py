@@ -4,7 +4,9 @@ used by the GPU tests are the derivatives of the forward ones."""
 
 from __future__ import annotations
 
+import ast
 import ctypes as C
+import pathlib
 import threading
 import weakref
 
@@ -201,6 +203,49 @@ def test_adamw_tables_and_step_count(backend):
     assert [first[5][i] for i in range(3)] == [g._data.ptr for g in gs]
     assert first[9:] == (0.1, 0.8, 0.95, 1e-6, 0.2, 1, None)
     assert second[9:] == (0.05, 0.8, 0.95, 1e-6, 0.2, 2, scale._data.ptr)
+
+
+def test_adamw_step_on_the_callers_lists(backend):
+    ps = [_arr(backend, 3, 4), _arr(backend, 5), _arr(backend, 0, 2)]
+    gs, m, v = ([_arr(backend, *p.shape) for p in ps] for _ in range(3))
+    scale = _arr(backend, 1)
+    before = backend._lib.next_ptr
+    pb.adamw_step(ps, gs, m, v, step=7, lr=0.1, betas=(0.8, 0.95), eps=1e-6, weight_decay=0.2, grad_scale=scale)
+    assert backend._lib.next_ptr == before  # nothing was allocated
+    args = _call(backend, "pb_adamw")
+    assert args[2:4] == (_lib.PB_F32, 3) and [args[8][i] for i in range(3)] == [12, 5, 0]
+    for table, arrays in zip(args[4:8], (ps, gs, m, v)):
+        assert [table[i] for i in range(3)] == [x._data.ptr for x in arrays]
+    assert args[9:] == (0.1, 0.8, 0.95, 1e-6, 0.2, 7, scale._data.ptr)
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(params=[]), ValueError), (dict(grads=[]), ValueError), (dict(exp_avg_sq=[None, None]), ValueError),
+    (dict(step=1.5), TypeError), (dict(betas=(0.9,)), ValueError), (dict(grads=lambda b: [_arr(b, 5)]), ValueError),
+    (dict(exp_avg=lambda b: [_arr(b, 4, dtype=np.float64)]), ValueError),
+    (dict(exp_avg=lambda b: [_released(b, 4)]), ValueError),
+    (dict(exp_avg=lambda b: [_arr(_backend(), 4)]), pb.BackendMismatchError),
+    (dict(grad_scale=lambda b: _arr(b, 2)), ValueError),
+])
+def test_adamw_step_refuses(backend, change, error):
+    backend._lib.pb_free = lambda *args: 0
+    args = {k: [_arr(backend, 4)] for k in ("params", "grads", "exp_avg", "exp_avg_sq")} | dict(step=1)
+    args |= {k: v(backend) if callable(v) else v for k, v in change.items()}
+    with pytest.raises(error):
+        pb.adamw_step(**args)
+    assert not [n for n, _ in backend._lib.calls if n == "pb_adamw"]
+
+
+def test_the_operator_cases_call_what_the_package_has():
+    """Every pacho_b200 name that the cases of perf/operators.py call is there."""
+    tree = ast.parse((pathlib.Path(__file__).parent.parent / "perf" / "operators.py").read_text())
+    aliases = {a.asname or a.name for n in ast.walk(tree) if isinstance(n, ast.Import) for a in n.names
+               if a.name == "pacho_b200"}
+    called = {n.attr for n in ast.walk(tree) if isinstance(n, ast.Attribute) and isinstance(n.value, ast.Name)
+              and n.value.id in aliases}
+    called |= {a.name for n in ast.walk(tree) if isinstance(n, ast.ImportFrom) and n.module == "pacho_b200"
+               for a in n.names}
+    assert called and not [name for name in called if not hasattr(pb, name)]
 
 
 def test_c_entries_refuse_before_any_device_call():
