@@ -15,7 +15,7 @@ import torch
 own = False
 
 _DTYPES = {"f32": torch.float32, "f64": torch.float64}
-_BETAS, _EPS_ADAM, _DECAY, _RATE, _STEPS = (0.9, 0.95), 1e-8, 0.1, 3e-4, 999
+_BETAS, _EPS_ADAM, _DECAY, _RATE, _STEP = (0.9, 0.95), 1e-8, 0.1, 3e-4, 1000
 _EPS_NORM = 1e-5
 _backend = None
 
@@ -165,17 +165,12 @@ def prepare(case, seed):
         s["m"] = normal(size).mul_(0.002).mul_(live)
         s["v"] = normal(size).square_().mul_(1e-4).mul_(live)
         s["scale"] = torch.rand(1, generator=gen, device="cuda", dtype=t) if case["scaled"] else None
-        s["steps"] = _STEPS
     if own:
         # The same tensors as the framework's arrays (no copy), as its user holds them.
         backend = _device()
         if case["op"] == "adamw":
-            from pacho_b200 import AdamW
-
-            p, g, m, v = ([backend.view(s[k][at:at + n]) for at, n in spans] for k in ("p", "g", "m", "v"))
-            s["dev"] = {"g": g, "scale": backend.view(s["scale"]) if case["scaled"] else None,
-                        "optimizer": AdamW(p, lr=_RATE, betas=_BETAS, eps=_EPS_ADAM, weight_decay=_DECAY,
-                                           exp_avg=m, exp_avg_sq=v, steps=_STEPS)}
+            s["dev"] = {k: [backend.view(s[k][at:at + n]) for at, n in spans] for k in ("p", "g", "m", "v")}
+            s["dev"]["scale"] = backend.view(s["scale"]) if case["scaled"] else None
         else:
             s["dev"] = {k: backend.view(x) for k, x in s.items() if isinstance(x, torch.Tensor)}
     return s
@@ -275,12 +270,11 @@ def _norm_grad(s):
 
 
 def _adamw(s):
-    s["steps"] += 1
     g = s["g"] * s["scale"] if s["scale"] is not None else s["g"]
     s["m"].mul_(_BETAS[0]).add_(g, alpha=1 - _BETAS[0])
     s["v"].mul_(_BETAS[1]).add_(g * g, alpha=1 - _BETAS[1])
-    root = torch.sqrt(s["v"] / (1 - _BETAS[1] ** s["steps"])) + _EPS_ADAM
-    s["p"].mul_(1 - _RATE * _DECAY).sub_(s["m"] / root, alpha=_RATE / (1 - _BETAS[0] ** s["steps"]))
+    root = torch.sqrt(s["v"] / (1 - _BETAS[1] ** _STEP)) + _EPS_ADAM
+    s["p"].mul_(1 - _RATE * _DECAY).sub_(s["m"] / root, alpha=_RATE / (1 - _BETAS[0] ** _STEP))
     return s["p"], s["m"], s["v"]
 
 
@@ -322,7 +316,8 @@ def _run_own(s):
         pb.group_norm_backward(d["dy"], d["x"], case["groups"], d["mean"], d["rstd"], d.get("weight"),
                                d.get("bias"), activation=act, out=(d["dx"], d.get("dweight"), d.get("dbias")))
         return {k: s[k] for k in (("dx", "dweight", "dbias") if case["affine"] else ("dx",))}
-    d["optimizer"].step(d["g"], grad_scale=d["scale"])
+    pb.adamw_step(d["p"], d["g"], d["m"], d["v"], step=_STEP, lr=_RATE, betas=_BETAS, eps=_EPS_ADAM,
+                  weight_decay=_DECAY, grad_scale=d["scale"])
     return {k: s[k] for k in ("p", "m", "v")}
 
 
@@ -367,7 +362,7 @@ def exact(case, seed):
     g = d["g"] * d["scale"] if case["scaled"] else d["g"]
     m = _BETAS[0] * d["m"] + (1 - _BETAS[0]) * g
     v = _BETAS[1] * d["v"] + (1 - _BETAS[1]) * g ** 2
-    fixed = [1 - np.float64(b) ** (_STEPS + 1) for b in _BETAS]
+    fixed = [1 - np.float64(b) ** _STEP for b in _BETAS]
     p = d["p"] - _RATE * (_DECAY * d["p"] + (m / float(fixed[0])) / ((v / float(fixed[1])) ** 0.5 + _EPS_ADAM))
     return {"p": p, "m": m, "v": v}
 
