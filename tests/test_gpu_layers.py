@@ -289,6 +289,35 @@ def test_group_norm_backward_where_the_mean_over_the_deviation_overflows(b200, s
             close(q.numpy(), v, e, np.float32, f"{act} {name}")
 
 
+def _scaled_inputs(shape, scale, seed):
+    n, s, c, g = shape
+    rng = np.random.default_rng(n + s + c + seed)
+    x = ((rng.standard_normal((n, s, c)) + 0.3) * scale).astype(np.float32)
+    w, b = (rng.standard_normal(c) * 0.3 + 1).astype(np.float32), (rng.standard_normal(c) * 0.3).astype(np.float32)
+    return x, w, b, rng
+
+
+# A shape of each kernel and way through it: rows in a part of a warp, a warp and a
+# block, of packs and of single values, of several positions; the ring with packs
+# and with single values; the samples kernel.
+KERNELS = [(300, 1, 24, 3), (130, 1, 512, 2), (20, 1, 4000, 1), (60, 1, 62, 2), (9, 1, 1022, 1), (3, 1, 8191, 1),
+           (17, 3, 1300, 26), (9, 3, 25, 1), (2, 4096, 20, 4), (3, 5000, 21, 3), (2, 150, 1921, 17), (2, 80, 2048, 8),
+           (3, 1, 8193, 1)]
+
+
+@pytest.mark.parametrize("scale,eps", [(1e30, 1e-5), (1e20, 0.0), (1e-15, 0.0), (1e-24, 0.0), (1e-30, 0.0)])
+@pytest.mark.parametrize("shape", KERNELS)
+def test_group_norm_of_values_whose_squares_leave_float32(b200, shape, scale, eps):
+    """Deviations of 1e20 and more or 1e-24 and less: mean, rstd and y are ordinary float32
+    values, the squares are not."""
+    x, w, b, _ = _scaled_inputs(shape, scale, 3)
+    for act in (None, "silu"):
+        got = pb.group_norm(up(b200, x), shape[3], up(b200, w), up(b200, b), eps=eps, activation=act)
+        want, bounds = ref.group_norm(x, shape[3], w, b, eps, act, 2.0 ** -24)
+        for name, q, v, e in zip(("y", "mean", "rstd"), got, want, bounds):
+            close(q.numpy(), v, e, np.float32, f"{act} {name}")
+
+
 @pytest.mark.parametrize("shape", [(4, 1, 64, 2), (3, 700, 8, 2)])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("where", [0, 5])
