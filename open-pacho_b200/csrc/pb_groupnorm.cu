@@ -112,15 +112,16 @@ constexpr int64_t kSharedChannels = 1024;
 
 // What a thread needs of its V channels c, c + step, ...: the sums of one pass over
 // positions.  Channels from C on have sums that nobody reads.
-// Backward, xhat = rstd d with d = x - mean, so the second sum is formed of
-// dz d and takes its factor rstd at the end.  Two positions at a time: their
-// terms are added in T and the pair in float64, which halves the conversions (they
-// share a unit of a sixteenth of the rate with the exponential) for one rounding more.
+// Backward, the second sum is of dz xhat, xhat = (x - mean) rstd: dz (x - mean), with
+// the factor rstd at the end, would leave float32's range where x is far from 1.
+// Two positions at a time: their terms are added in T and the pair in float64, which
+// halves the conversions (they share a unit of a sixteenth of the rate with the
+// exponential) for one rounding more.
 template <typename T, int V, int ACT, bool BWD>
 struct ChannelSums {
   double s1[V], s2[V];
   double k[BWD ? 1 : V];
-  T mean[BWD ? V : 1], rstd[BWD ? V : 1], rw[BWD ? V : 1], b[BWD ? V : 1];
+  T mean[BWD ? V : 1], rstd[BWD ? V : 1], w[BWD ? V : 1], b[BWD ? V : 1];
 
   __device__ __forceinline__ void begin(const NormArgs<T>& p, int64_t n, int64_t c, bool on, int step = 1) {
 #pragma unroll
@@ -132,7 +133,7 @@ struct ChannelSums {
       if constexpr (BWD) {
         mean[i] = __ldg(p.mean + n * p.G + g);
         rstd[i] = __ldg(p.rstd + n * p.G + g);
-        rw[i] = here && p.weight ? rstd[i] * __ldg(p.weight + ch) : rstd[i];
+        w[i] = here && p.weight ? __ldg(p.weight + ch) : T(1);
         b[i] = here && p.bias ? __ldg(p.bias + ch) : T(0);
       } else {
         k[i] = shift_of(p, n, g);
@@ -140,9 +141,9 @@ struct ChannelSums {
     }
   }
   __device__ __forceinline__ void term(int i, T x, T dy, T* dz, T* product) const {
-    const T d = x - mean[i];
-    *dz = dy * slope<T, ACT>(fma(d, rw[i], b[i]));
-    *product = *dz * d;
+    const T xhat = (x - mean[i]) * rstd[i];
+    *dz = dy * slope<T, ACT>(fma(xhat, w[i], b[i]));
+    *product = *dz * xhat;
   }
   // Backward, dy becomes dz.
   __device__ __forceinline__ void add(const Pack<T, V>& x, Pack<T, V>& dy) {
@@ -178,34 +179,29 @@ struct ChannelSums {
       add(x1, dy1);
     }
   }
-  __device__ __forceinline__ void end() {
-    if constexpr (BWD) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) s2[i] *= (double)rstd[i];
-    }
-  }
 };
 
-// ... and its results, y = act(d rw + b) with rw = rstd w, and
-// dx = rstd (w dz - m1 - xhat m2) = rw dz - rstd m1 - d rstd^2 m2.
+// ... and its results, y = act((x - mean) rw + b) with rw = rstd w, and
+// dx = rstd (w dz - m1 - xhat m2).  Backward every factor stays apart: rstd^2 m2 leaves
+// float32's range where x is far from 1, and z has the bits that the sums had.
 template <typename T, int V, int ACT, bool BWD>
 struct ChannelResults {
-  T mean[V], rw[V], b[V];
-  T r1[V];                 // backward: -rstd m1; forward: the mean's low part, so that its rounding does not show
-  T r2[BWD ? V : 1];       // -rstd^2 m2
+  T mean[V], w[V], b[V];   // forward: w becomes rw
+  T r1[V];                 // backward: -m1; forward: the mean's low part, so that its rounding does not show
+  T rstd[BWD ? V : 1], r2[BWD ? V : 1];  // r2 = -m2
 
-  // What does not depend on the sums of sample n; backward rw is rstd until `end`.
+  // What does not depend on the sums of sample n.
   __device__ __forceinline__ void begin(const NormArgs<T>& p, int64_t n, int64_t c, bool on, int step = 1) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int64_t ch = c + i * step;
       const bool here = on && ch < p.C;
-      r1[i] = here && p.weight ? __ldg(p.weight + ch) : T(1);
+      w[i] = here && p.weight ? __ldg(p.weight + ch) : T(1);
       b[i] = here && p.bias ? __ldg(p.bias + ch) : T(0);
       if constexpr (BWD) {
         const int64_t g = here ? fdiv(ch, p.by_m) : 0;
         mean[i] = __ldg(p.mean + n * p.G + g);
-        rw[i] = __ldg(p.rstd + n * p.G + g);
+        rstd[i] = __ldg(p.rstd + n * p.G + g);
       }
     }
   }
@@ -217,37 +213,36 @@ struct ChannelResults {
       const int64_t ch = c + i * step;
       const int64_t g = on && ch < p.C ? fdiv(ch, p.by_m) : 0;
       const double2 t = stats ? stats[g] : __ldcg(p.group + n * p.G + g);
-      const double w = (double)r1[i];
       if constexpr (BWD) {
-        const double r = (double)rw[i];
-        rw[i] = (T)(r * w);
-        r1[i] = (T)(-r * t.x);
-        r2[i] = (T)(-r * r * t.y);
+        r1[i] = (T)-t.x;
+        r2[i] = (T)-t.y;
       } else {
         mean[i] = (T)t.x;
         r1[i] = (T)(t.x - (double)mean[i]);
-        rw[i] = (T)(t.y * w);
+        w[i] = (T)(t.y * (double)w[i]);
       }
     }
   }
-  // dx where dz is known.
+  // dx where dz and xhat are known.
+  __device__ __forceinline__ T gradient(int i, T dz, T xhat) const {
+    return rstd[BWD ? i : 0] * fma(w[i], dz, fma(xhat, r2[BWD ? i : 0], r1[i]));
+  }
   __device__ __forceinline__ Pack<T, V> of_dz(const Pack<T, V>& x, const Pack<T, V>& dz) const {
     Pack<T, V> o;
 #pragma unroll
-    for (int i = 0; i < V; ++i) o.v[i] = fma(rw[i], dz.v[i], fma(x.v[i] - mean[i], r2[BWD ? i : 0], r1[i]));
+    for (int i = 0; i < V; ++i) o.v[i] = gradient(i, dz.v[i], (x.v[i] - mean[i]) * rstd[BWD ? i : 0]);
     return o;
   }
   __device__ __forceinline__ Pack<T, V> of(const Pack<T, V>& x, const Pack<T, V>& dy) const {
     Pack<T, V> o;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      T d = x.v[i] - mean[i];
+      const T d = x.v[i] - mean[i];
       if constexpr (BWD) {
-        const T dz = dy.v[i] * slope<T, ACT>(fma(d, rw[i], b[i]));
-        o.v[i] = fma(rw[i], dz, fma(d, r2[i], r1[i]));
+        const T xhat = d * rstd[i];
+        o.v[i] = gradient(i, dy.v[i] * slope<T, ACT>(fma(xhat, w[i], b[i])), xhat);
       } else {
-        d -= r1[i];
-        o.v[i] = activate<T, ACT>(fma(d, rw[i], b[i]));
+        o.v[i] = activate<T, ACT>(fma(d - r1[i], w[i], b[i]));
       }
     }
     return o;
@@ -334,7 +329,6 @@ __device__ __forceinline__ void sums_item(const NormArgs<T>& p, int64_t unit, in
         sums.add(x, dy);
       }
     }
-    sums.end();
     sum_rows<T, V, true>(p, sums, c0, tx, ty, red, out, BWD && p.chan ? p.chan + unit * p.C : nullptr);
   }
   sum_groups<T, BWD>(p, out, p.part + unit * p.G);
@@ -669,8 +663,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1) norm_ring_kernel(const N
         take(turn + k, k, n, true, k >= stages - held, k < stages - held,
              [&](P x0, D d0, P x1, D d1, int64_t, int64_t) { sums.add2(x0, d0, x1, d1); },
              [&](P x, D dy, int64_t) { sums.add(x, dy); });
-      sums.end();
-      // Over the rows of threads: red is [ty][tx * V], `parts` threads per channel.
+        // Over the rows of threads: red is [ty][tx * V], `parts` threads per channel.
       if (on) {
 #pragma unroll
         for (int i = 0; i < V; ++i) red[(ly * V + i) * tx + lx] = make_double2(sums.s1[i], sums.s2[i]);
@@ -1008,7 +1001,7 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, kRowBlocks<V * ITEMS * siz
         });
       }
     } else {
-      // x becomes x - mean, e becomes w dz.  The row's sums go pair by pair in T and
+      // x becomes xhat, e becomes w dz.  The row's sums go pair by pair in T and
       // then in float64 (see ChannelSums).  Packs and rows that are not there have
       // dy = 0, and mean and rstd of 0 so that 0 times them cannot be NaN.
       double2 t = make_double2(0.0, 0.0);
@@ -1029,11 +1022,11 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, kRowBlocks<V * ITEMS * siz
             T z = T(0), q = T(0);
 #pragma unroll
             for (int j = i; j < i + (V > 1 ? 2 : 1); ++j) {
-              const T d = x[k].v[j] - mu, xh = d * r;
+              const T xh = (x[k].v[j] - mu) * r;
               const T dz = e[k].v[j] * slope<T, decltype(which)::value>(fma(xh, w[j], b[j])), product = dz * xh;
               db[k][j] += (Sum)dz;
               dw[k][j] += (Sum)product;
-              x[k].v[j] = d;
+              x[k].v[j] = xh;
               e[k].v[j] = w[j] * dz;
               z = j == i ? e[k].v[j] : z + e[k].v[j];
               q = j == i ? w[j] * product : fma(w[j], product, q);
@@ -1056,8 +1049,8 @@ __global__ void __launch_bounds__(kRowThreads<LANES>, kRowBlocks<V * ITEMS * siz
         }
       }
       t = row_sum<LANES>(t);
-      // dx = rstd (w dz - m1 - xhat m2), xhat = d rstd.
-      const T m1 = (T)(t.x * share), m2 = (T)(t.y * share * (double)rstd);
+      // dx = rstd (w dz - m1 - xhat m2)
+      const T m1 = (T)(t.x * share), m2 = (T)(t.y * share);
       if (n < n1) {
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k) {

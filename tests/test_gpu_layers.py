@@ -318,6 +318,30 @@ def test_group_norm_of_values_whose_squares_leave_float32(b200, shape, scale, ep
             close(q.numpy(), v, e, np.float32, f"{act} {name}")
 
 
+@pytest.mark.parametrize("scale", [1e30, 1e22, 1e-22, 1e-30])
+@pytest.mark.parametrize("size", [1.0, 1e10, 1e-10])
+@pytest.mark.parametrize("shape", KERNELS)
+def test_group_norm_backward_of_large_and_small_values(b200, shape, size, scale):
+    """rstd far from 1: dx is of the size of dy rstd, while rstd^2 and dy (x - mean) leave
+    float32's range on one side or the other.  dy = 1e10 at rstd = 1e30 is beyond it
+    itself: such a dx is the infinity of its sign."""
+    x, w, b, rng = _scaled_inputs(shape, scale, 4)
+    g = shape[3]
+    dy = (rng.standard_normal(x.shape) * size).astype(np.float32)
+    (_, mean, rstd), _ = ref.group_norm(x, g, w, b, 0.0, None, 0.0)
+    mean, rstd = mean.astype(np.float32), rstd.astype(np.float32)
+    for act in (None, "silu"):
+        got = pb.group_norm_backward(*(up(b200, v) for v in (dy, x)), g, *(up(b200, v) for v in (mean, rstd, w, b)),
+                                     activation=act)
+        want, bounds = ref.group_norm_backward(dy, x, g, mean, rstd, w, b, act, 2.0 ** -24)
+        for name, q, v, e in zip(("dx", "dweight", "dbias"), got, want, bounds):
+            q, most = q.numpy(), float(np.finfo(np.float32).max)
+            beyond = np.abs(v) - FACTOR * e > most
+            assert np.array_equal(q[beyond], np.sign(v[beyond]) * np.float32(np.inf)), f"{act} {name}"
+            here = np.abs(v) + FACTOR * e <= most
+            close(q[here], v[here], e[here], np.float32, f"{act} {name}")
+
+
 @pytest.mark.parametrize("shape", [(4, 1, 64, 2), (3, 700, 8, 2)])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("where", [0, 5])
