@@ -49,21 +49,34 @@ struct NormArgs {
   double eps;
 };
 
-// Phi(z), the normal distribution's, and phi(z), its density.
+// Phi(z), the normal distribution's, and phi(z), its density, each to a few roundings
+// of its own size wherever the density is a normal number.
 //
-// float32: Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26: erfc(x) =
-// (a1 t + ... + a5 t^5) e^(-x^2), t = 1 / (1 + p x), within 1.5e-7 for x >= 0; with x =
-// |z| / sqrt 2 the exponential is that of phi, and Phi is off by 7.5e-8 at most, little
-// more than a rounding of its largest values.  erfcf takes four times as long.
+// float32: Phi(-a) = phi(a) R(a) for a >= 0, with Mills' ratio R as a polynomial in
+// t = 1 / (1 + p a), the form of Abramowitz and Stegun, Handbook of Mathematical
+// Functions, 7.1.26, of degree 8 and with coefficients fitted to R on [0, 20] for the least
+// relative error, 8.6e-8.  The density's exponent is formed in two parts, as in
+// sigmoid_pair: the roundings of z^2 and of its product would be z^2 of the result's.
+// Beyond |z| = 20 the density is zero; the minimum keeps a NaN.  32768 x 2048 forward: 145 us;
+// 7.1.26 itself, off by 1e-3 of Phi at z = -5, 130; erfcf and expf, off by z^2 roundings, 198.
 __device__ __forceinline__ void normal(float z, float* Phi, float* phi) {
-  const float x = fabsf(z) * 0.70710678f;
-  const float e = exp2_unit(z * z * -0.72134752f);  // e^(-z^2 / 2)
-  const float t = reciprocal_unit(fmaf(0.3275911f, x, 1.0f));
-  float q = fmaf(1.061405429f, t, -1.453152027f);
-  q = fmaf(q, t, 1.421413741f);
-  q = fmaf(q, t, -0.284496736f);
-  q = fmaf(q, t, 0.254829592f);
-  const float tail = 0.5f * q * t * e;
+  constexpr float kHalfLog2e = 0.721347511f, kHalfLog2eLow = 9.62981515e-9f, kLn2 = 0.693147182f;
+  float a;
+  asm("min.NaN.f32 %0, %1, 0f41A00000;" : "=f"(a) : "f"(fabsf(z)));
+  const float s = a * a, k = s * -kHalfLog2e;
+  const float r = fmaf(-s, kHalfLog2eLow, fmaf(fmaf(a, a, -s), -kHalfLog2e, fmaf(-s, kHalfLog2e, -k)));
+  float e = exp2_unit(k);  // e^(-z^2 / 2)
+  e = fmaf(e, r * kLn2, e);
+  const float t = reciprocal_unit(fmaf(0.3f, a, 1.0f));
+  float q = fmaf(0.0376731381f, t, -0.166167408f);
+  q = fmaf(q, t, 0.223319471f);
+  q = fmaf(q, t, -0.0713290721f);
+  q = fmaf(q, t, 0.139563337f);
+  q = fmaf(q, t, 0.0957120657f);
+  q = fmaf(q, t, 0.121712156f);
+  q = fmaf(q, t, 0.119510069f);
+  q = fmaf(q, t, 6.19924685e-06f);
+  const float tail = q * e;
   *Phi = z < 0.0f ? tail : 1.0f - tail;
   *phi = e * 0.39894228f;
 }

@@ -342,6 +342,32 @@ def test_group_norm_backward_of_large_and_small_values(b200, shape, size, scale)
             close(q[here], v[here], e[here], np.float32, f"{act} {name}")
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_gelu_keeps_its_relative_accuracy(b200, dtype):
+    """With weights of zero an activation is of the bias alone.  From -12 on, where the
+    density is a normal float32, z Phi(z) is off by ACT roundings of itself, and its slope
+    Phi + z phi of the two terms.  In float64 the argument of erfc, z over the root of 2, has two
+    roundings in the kernel and two in the definition; erfc(x) passes on 2 x^2 = z^2 of
+    each, and exp(-z^2 / 2) as many."""
+    b = np.concatenate([np.linspace(-12, 12, 4001), np.linspace(-0.3, 0.3, 800), [0.0]]).astype(dtype)
+    c = b.size
+    rng = np.random.default_rng(5)
+    u = ref.U[np.dtype(dtype)]
+    z = b.astype(np.float64)
+    k = u * (ref.ACT + (4 * z * z if dtype == np.float64 else 0))
+    x = rng.standard_normal((1, 1, c)).astype(dtype)
+    y, _, _ = pb.group_norm(up(b200, x), 1, up(b200, np.zeros(c, dtype)), up(b200, b), activation="gelu")
+    want = ref.activate(z, "gelu")
+    close(y.numpy()[0, 0], want, k * np.abs(want), dtype, "gelu")
+    stats = [up(b200, v) for v in (np.zeros((1, 1), dtype), np.ones((1, 1), dtype))]
+    dy = rng.standard_normal((1, 1, c)).astype(dtype)
+    _, _, dbias = pb.group_norm_backward(up(b200, dy), up(b200, x), 1, *stats, up(b200, np.zeros(c, dtype)), up(b200, b),
+                                         activation="gelu")
+    terms = np.abs(ref._erfc(-z / np.sqrt(2.0)) / 2) + np.abs(z) * np.exp(-z * z / 2) / np.sqrt(2 * np.pi)
+    g = dy[0, 0].astype(np.float64)
+    close(dbias.numpy(), g * ref.slope(z, "gelu"), k * np.abs(g) * terms, dtype, "slope")
+
+
 @pytest.mark.parametrize("shape", [(4, 1, 64, 2), (3, 700, 8, 2)])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("where", [0, 5])
