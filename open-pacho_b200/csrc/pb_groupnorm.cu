@@ -1335,6 +1335,34 @@ int launch_act(Device* d, int act, const NormArgs<T>& p) {
   }
 }
 
+// Whether a group that fits the registers of a block is read there, once, rather than by
+// the ring.  Times in us, rows and ring, silu, float32.
+template <typename T, bool BWD>
+bool rows_pay(Device* d, const NormArgs<T>& p) {
+  if (p.S == 1 || !ring_takes(p)) return true;
+  const int64_t run = p.m * (int64_t)sizeof(T), sample = p.S * p.C * (int64_t)sizeof(T);
+  const double rounds = (double)ceil_div(p.N, (int64_t)d->sm_count);
+  const bool sums = BWD && (p.dweight || p.dbias);
+  // Runs of less than the 32 bytes that memory moves at once: the rows read some 0.6 TB/s
+  // (1.3 from 16 bytes on) and the ring, which copies whole positions, 4, but it takes 6.5 us
+  // more for each round of a sample per block.  Forward, groups of one channel: 16 x 512 x 64
+  // 10.6 and 12.7, 8 x 4096 x 320 163 and 31, 1000 x 64 x 640 495 and 118 (of four 154 and 101),
+  // 10000 x 64 x 64 402 and 380, 40000 x 65 x 32 849 and 1385.  Gradients with sums for each
+  // position: 2000 x 200 x 32 of four 166 and 118, 20000 x 100 x 64 2033 and 1002.
+  if (run < 32) {
+    if (sums && p.S > 64) return false;
+    const double moved = (BWD ? 3.0 : 2.0) * (double)p.N * (double)sample;
+    return moved / (run < 16 ? 0.6e6 : 1.3e6) <= 10.0 + 6.5 * rounds + moved / 4e6;
+  }
+  // The rows give a row of sums for dweight and dbias for each position: with many
+  // positions the ring's sums of whole runs are less to add up, unless it takes many
+  // rounds over small samples.  Gradients, groups of eight: 1000 x 64 x 256 73 and 85, 1000 x 65 x
+  // 256 114 and 85, 148 x 65 x 64 46 and 16, 1500 x 100 x 64 89 and 95, 5000 x 65 x 64 126 and 253, 20000 x
+  // 128 x 64 546 and 1087, 5000 x 65 x 256 510 and 352.
+  if (!sums) return true;
+  return p.S <= 64 || (p.S <= 128 && rounds > 8 && sample <= kRowPacks * 16);
+}
+
 struct Pointers {
   const void *x, *dy, *weight, *bias;
   void *out, *mean, *rstd, *dweight, *dbias;
@@ -1360,13 +1388,8 @@ int dispatch(Device* d, int act, int64_t N, int64_t S, int64_t C, int64_t G, dou
   p.eps = eps;
   constexpr int V = Vec16<T>::n;
   const bool aligned = (((uintptr_t)q.x | (uintptr_t)q.dy | (uintptr_t)q.out | (uintptr_t)q.weight | (uintptr_t)q.bias) & 15) == 0;
-  // A group that fits the registers of a block is read once.  It then gives a row of
-  // sums for dweight and dbias per position: with many positions the ring's sums of
-  // whole runs are less to add up (float32 backward, rows and ring: 16 x 64 x 1280 in 32
-  // groups 19 and 23 us, 16 x 300 x 640 in 32 42 and 27, 32 x 8000 x 8 in 8 876 and 23).
-  const bool packed = aligned && p.m % V == 0, by_rows = !BWD || S <= 64 || !(q.dweight || q.dbias) || !ring_takes(p);
-  if (by_rows && S <= kRowPacks * V && S * C < (int64_t(1) << 31) && S * p.m <= kRowPacks * V)
-    return packed ? launch_rows_of<T, V, BWD>(d, act, p) : launch_rows_of<T, 1, BWD>(d, act, p);
+  if (S <= kRowPacks * V && S * C < (int64_t(1) << 31) && S * p.m <= kRowPacks * V && rows_pay<T, BWD>(d, p))
+    return aligned && p.m % V == 0 ? launch_rows_of<T, V, BWD>(d, act, p) : launch_rows_of<T, 1, BWD>(d, act, p);
   return aligned && C % V == 0 ? launch_act<T, V, BWD>(d, act, p) : launch_act<T, 1, BWD>(d, act, p);
 }
 

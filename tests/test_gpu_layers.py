@@ -450,6 +450,61 @@ def test_group_norm_backward_of_arrays_that_start_anywhere(b200, shape, odd):
         assert np.all(got[:at[k]] == 7) and np.all(got[at[k] + v.size:] == 7)
 
 
+def _check_group_norm(b200, shape, dtype):
+    """Forward and backward of one shape with weight, bias and silu."""
+    x, w, b, rng = _norm_inputs(shape, dtype, 6)
+    g = shape[3]
+    dy = rng.standard_normal(x.shape).astype(dtype)
+    dx, dw, db, ddy = (up(b200, v) for v in (x, w, b, dy))
+    out = tuple(poisoned(b200, v, dtype) for v in (x.shape, (shape[0], g), (shape[0], g)))
+    got = pb.group_norm(dx, g, dw, db, eps=1e-3, activation="silu", out=out)
+    want, bounds = ref.group_norm(x, g, w, b, 1e-3, "silu", ref.U[np.dtype(dtype)])
+    for name, q, v, e in zip(("y", "mean", "rstd"), got, want, bounds):
+        close(q.numpy(), v, e, dtype, name)
+    mean, rstd = (v.astype(dtype) for v in want[1:])
+    out = tuple(poisoned(b200, v.shape, dtype) for v in (x, w, b))
+    got = pb.group_norm_backward(ddy, dx, g, up(b200, mean), up(b200, rstd), dw, db, activation="silu", out=out)
+    want, bounds = ref.group_norm_backward(dy, x, g, mean, rstd, w, b, "silu", ref.U[np.dtype(dtype)])
+    for name, q, v, e in zip(("dx", "dweight", "dbias"), got, want, bounds):
+        close(q.numpy(), v, e, dtype, name)
+
+
+# Shapes on either side of the choice between rows and ring: samples of few positions and
+# many rounds, short runs.
+CHOICES = [(1300, 70, 32, 4), (1300, 129, 8, 1), (1100, 65, 32, 4), (30, 600, 64, 64), (60, 64, 256, 256),
+           (60, 64, 256, 64), (4, 4096, 33, 33), (9, 65, 48, 6), (2, 2000, 96, 24)]
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("shape", CHOICES)
+def test_group_norm_on_either_side_of_a_choice(b200, shape, dtype):
+    _check_group_norm(b200, shape, dtype)
+
+
+@pytest.mark.parametrize("shape,backward", [((20000, 65, 32, 4), True), ((40000, 65, 32, 1), True),
+                                            ((8, 4096, 320, 320), False), ((16, 8192, 64, 64), False),
+                                            ((1000, 64, 640, 640), False), ((1000, 64, 640, 640), True)])
+def test_group_norm_does_not_fall_to_a_tenth_of_the_copy_rate(b200, shape, backward):
+    """A wrong choice of the kernel takes 10 to 20 times what the bytes need at 6.4 TB/s on
+    these, the right one 2 to 4."""
+    n, s, c, g = shape
+    x, y, dy = (DeviceArray(b200, b200.full((n, s, c), v, np.float32), (n, s, c), np.float32) for v in (0.5, 0, 1))
+    w, b, dw, db = (DeviceArray(b200, b200.full((c,), 1, np.float32), (c,), np.float32) for _ in range(4))
+    mean, rstd = (DeviceArray(b200, b200.full((n, g), 0.5, np.float32), (n, g), np.float32) for _ in range(2))
+    lib, ctx, best = b200._lib, b200._ctx, np.inf
+    for _ in range(6):
+        ms = C.c_float()
+        _lib.check(lib.pb_timer_start(ctx, 0))
+        if backward:
+            pb.group_norm_backward(dy, x, g, mean, rstd, w, b, activation="silu", out=(y, dw, db))
+        else:
+            pb.group_norm(x, g, w, b, activation="silu", out=(y, mean, rstd))
+        _lib.check(lib.pb_timer_stop(ctx, 0, C.byref(ms)))
+        best = min(best, ms.value * 1e3)
+    floor = (3 if backward else 2) * n * s * c * 4 / 6.4e6
+    assert best <= 7 * floor, f"{best:.1f} us for {floor:.1f}"
+
+
 def test_group_norm_repeats_its_bits(b200):
     for shape in ((500, 1, 256, 4), (3, 5000, 24, 3)):
         x, w, b, rng = _norm_inputs(shape, np.float32)
