@@ -1168,8 +1168,8 @@ int launch_rows(Device* d, int act, NormArgs<T> p) {
   PB_CHECK(kt_begin(d));
   norm_rows_kernel<T, V, LANES, ITEMS, BWD, FLAT><<<(unsigned)blocks, kRowThreads<LANES>, smem, d->stream>>>(p, act);
   PB_LAUNCHED(d);
-  PB_CHECK(kt_end(d));
-  return sums ? launch_affine<T>(d, p.part, p.chunks * p.S, p) : PB_OK;
+  if (sums) PB_CHECK(launch_affine<T>(d, p.part, p.chunks * p.S, p));
+  return kt_end(d);
 }
 
 // Packs of 16 bytes of a row that fit the rows kernel.
@@ -1268,8 +1268,8 @@ int launch_items(Device* d, NormArgs<T> p, int tx, int ty) {
   norm_samples_kernel<T, V, ACT, BWD>
       <<<(unsigned)grid, kThreads, 0, d->stream>>>(p, tx, ty, (unsigned)units, (unsigned)lead);
   PB_LAUNCHED(d);
-  PB_CHECK(kt_end(d));
-  return BWD && (p.dweight || p.dbias) ? launch_affine<T>(d, p.chan, units, p) : PB_OK;
+  if (BWD && (p.dweight || p.dbias)) PB_CHECK(launch_affine<T>(d, p.chan, units, p));
+  return kt_end(d);
 }
 
 template <typename T, int V, int ACT, bool BWD, bool SPREAD>
@@ -1307,8 +1307,8 @@ int launch_ring(Device* d, NormArgs<T> p) {
   PB_CUDA(cudaLaunchCooperativeKernel(kernel, dim3((unsigned)(together * p.chunks)), dim3(kRingThreads + 32), args,
                                       bytes, d->stream));
   PB_LAUNCHED(d);
-  PB_CHECK(kt_end(d));
-  return BWD && (p.dweight || p.dbias) ? launch_affine<T>(d, p.chan, together * p.chunks, p) : PB_OK;
+  if (BWD && (p.dweight || p.dbias)) PB_CHECK(launch_affine<T>(d, p.chan, together * p.chunks, p));
+  return kt_end(d);
 }
 
 // The ring takes rows that its threads span, of whole 16-byte pieces or not.

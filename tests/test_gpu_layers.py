@@ -505,6 +505,30 @@ def test_group_norm_does_not_fall_to_a_tenth_of_the_copy_rate(b200, shape, backw
     assert best <= 7 * floor, f"{best:.1f} us for {floor:.1f}"
 
 
+def test_the_kernel_timer_counts_the_sums_of_dweight(b200):
+    """Many rows of sums for few channels: adding them up is most of the call."""
+    n, s, c, g = 2048, 64, 8, 1
+    x, y, dy = (DeviceArray(b200, b200.full((n, s, c), v, np.float32), (n, s, c), np.float32) for v in (0.5, 0, 1))
+    w, dw = (DeviceArray(b200, b200.full((c,), 1, np.float32), (c,), np.float32) for _ in range(2))
+    mean, rstd = (DeviceArray(b200, b200.full((n, g), 0.5, np.float32), (n, g), np.float32) for _ in range(2))
+    lib, ctx = b200._lib, b200._ctx
+    whole, kernels, count, ms = np.inf, np.inf, C.c_uint64(), C.c_float()
+    for timed in [False] * 4 + [True] * 4:
+        total = C.c_double()
+        _lib.check(lib.pb_ktimer_enable(ctx, 0, 2 if timed else 0))
+        _lib.check(lib.pb_timer_start(ctx, 0))
+        pb.group_norm_backward(dy, x, g, mean, rstd, w, out=(y, dw, None))
+        _lib.check(lib.pb_timer_stop(ctx, 0, C.byref(ms)))
+        if timed:
+            _lib.check(lib.pb_ktimer_read(ctx, 0, C.byref(total), C.byref(count)))
+            assert count.value == 1
+            kernels = min(kernels, total.value)
+        else:
+            whole = min(whole, ms.value)
+    _lib.check(lib.pb_ktimer_enable(ctx, 0, 0))
+    assert kernels >= whole / 2, (kernels, whole)
+
+
 def test_group_norm_repeats_its_bits(b200):
     for shape in ((500, 1, 256, 4), (3, 5000, 24, 3)):
         x, w, b, rng = _norm_inputs(shape, np.float32)
