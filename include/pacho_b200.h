@@ -120,10 +120,10 @@ int pb_launch_count(pb_ctx* ctx, int dev, uint64_t* count);
 /* Per-kernel timer for rooflines: while enabled, every entry point brackets
  * its main kernel (the GEMM tile kernel, the GEMV/DOT/norm/elementwise/
  * reduction kernel -- not the operand-split or partial-merge helpers; a layer's
- * call with all of its kernels) with CUDA events on the device stream.  pb_ktimer_read waits for the stream,
- * returns the summed milliseconds and the number of bracketed launches since
- * the last enable/read, and starts a new count.  At most 4096 launches are
- * kept between reads (PB_ERR_UNSUPPORTED beyond).  An event between two
+ * call with all of its kernels) with CUDA events on the device stream.
+ * pb_ktimer_read waits for the stream, returns the summed milliseconds and the
+ * number of bracketed launches since the last enable/read, and starts a new
+ * count.  At most 4096 launches are kept between reads (PB_ERR_UNSUPPORTED beyond).  An event between two
  * chained launches serialises them, so time the whole step with the timer off.
  * enable = 2 is for a captured step: the event pairs become nodes of the graph,
  * each replay re-records them, and a read returns the last replay's times

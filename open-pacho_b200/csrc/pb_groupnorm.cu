@@ -21,6 +21,8 @@
 // sums and writes the result.  Such a part of the block stays with one group and
 // walks over the samples, so that weight and bias stay in registers and the sums of
 // dweight and dbias are its own.
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "pb_layers.cuh"
@@ -1151,6 +1153,10 @@ int launch_rows(Device* d, int act, NormArgs<T> p) {
   const bool sums = BWD && (p.dweight || p.dbias);
   int64_t most = ceil_div(p.N, (int64_t)SUBS * (sums ? 16 : 1));
   if (sums && most * p.G < wave) most = ceil_div(p.N, (int64_t)SUBS * 2);
+  // With S > 1 a unit writes S rows of sums, which take norm_affine_kernel 6 ns each, and a
+  // sample takes a unit 1.5 us: the least of 1.5 N / (SUBS chunks) + 0.006 S chunks.  2048 x 64 x 8
+  // 57 us, 418 with a unit for every two samples; 100 x 64 x 256 23 and 29; 16 x 64 x 1280 19 and 19.
+  if (sums && p.S > 1) most = std::min(most, (int64_t)std::ceil(std::sqrt(240.0 * (double)p.N / (double)(p.S * SUBS))));
   if (chunks > most) chunks = most;
   p.rows = ceil_div(p.N, chunks);
   p.chunks = ceil_div(p.N, p.rows);

@@ -481,6 +481,12 @@ def test_group_norm_on_either_side_of_a_choice(b200, shape, dtype):
     _check_group_norm(b200, shape, dtype)
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("shape", [(2048, 64, 8, 1), (300, 33, 100, 5), (60, 2, 16, 2), (3, 64, 8, 1)])
+def test_group_norm_of_many_samples_of_few_positions(b200, shape, dtype):
+    _check_group_norm(b200, shape, dtype)
+
+
 @pytest.mark.parametrize("shape,backward", [((20000, 65, 32, 4), True), ((40000, 65, 32, 1), True),
                                             ((8, 4096, 320, 320), False), ((16, 8192, 64, 64), False),
                                             ((1000, 64, 640, 640), False), ((1000, 64, 640, 640), True)])
