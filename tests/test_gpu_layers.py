@@ -535,6 +535,21 @@ def test_the_kernel_timer_counts_the_sums_of_dweight(b200):
     assert kernels >= whole / 2, (kernels, whole)
 
 
+# (N, S, C, G) of the ring's further ways: sums of more blocks and groups than each
+# block adds up for itself (8192, or 512 groups), with packs and with single values; and
+# several rounds of samples, the per-block sums of dweight and dbias carried on.
+RINGS = [((1, 20000, 64, 64), np.float32), ((1, 20000, 64, 64), np.float64), ((1, 9000, 1200, 600), np.float32),
+         ((1, 9000, 640, 640), np.float64), ((1, 20000, 65, 65), np.float32), ((1, 9000, 1201, 1201), np.float32),
+         ((1, 5000, 701, 701), np.float64), ((300, 200, 48, 1), np.float32), ((300, 200, 49, 1), np.float32),
+         ((40, 2000, 160, 8), np.float32), ((40, 1000, 160, 8), np.float64), ((700, 700, 13, 1), np.float32),
+         ((200, 400, 13, 1), np.float64)]
+
+
+@pytest.mark.parametrize("shape,dtype", RINGS)
+def test_group_norm_in_rounds_and_with_many_group_sums(b200, shape, dtype):
+    _check_group_norm(b200, shape, dtype)
+
+
 def test_group_norm_repeats_its_bits(b200):
     for shape in ((500, 1, 256, 4), (3, 5000, 24, 3)):
         x, w, b, rng = _norm_inputs(shape, np.float32)
@@ -688,6 +703,16 @@ def test_a_capture_that_would_grow_a_workspace_is_refused(b200):
             pass
     except NotImplementedError as exc:
         assert "grow" in str(exc)
+    pb.group_norm(x, 4, out=out)
+    assert np.all(out[0].numpy() == 0)
+
+
+def test_a_capture_that_grows_a_workspace_raises(b200):
+    x = up(b200, np.ones((3, 40000, 96), np.float32))
+    out = tuple(poisoned(b200, v, np.float32) for v in (x.shape, (3, 4), (3, 4)))
+    b200.release_cached_memory()
+    with pytest.raises(NotImplementedError, match="grow"):
+        b200.capture(lambda: pb.group_norm(x, 4, out=out))
     pb.group_norm(x, 4, out=out)
     assert np.all(out[0].numpy() == 0)
 
