@@ -336,13 +336,15 @@ class AdamW:
     def step(self, grads, *, grad_scale=None):
         """One step with a gradient array per parameter (shape and dtype of
         the parameter) and ``grad_scale`` as of :func:`adamw_step`."""
-        for arrays, known in zip((self.params, self.exp_avg, self.exp_avg_sq), self._known):
-            if [x._data.ptr for x in arrays] != known:
-                raise ValueError("the memory of a parameter or moment has been released or replaced")
-        p, m, v = self._tables
-        _adamw(self._backend, self._dtype, self._code, (p, self._table("grads", grads), m, v), self._sizes, grad_scale,
-               self.lr, self.betas, self.eps, self.weight_decay, self.steps + 1)
-        self.steps += 1
+        # One step at a time, its number with it: threads that share an optimizer.
+        with self._backend._lock:
+            for arrays, known in zip((self.params, self.exp_avg, self.exp_avg_sq), self._known):
+                if [x._data.ptr for x in arrays] != known:
+                    raise ValueError("the memory of a parameter or moment has been released or replaced")
+            p, m, v = self._tables
+            _adamw(self._backend, self._dtype, self._code, (p, self._table("grads", grads), m, v), self._sizes,
+                   grad_scale, self.lr, self.betas, self.eps, self.weight_decay, self.steps + 1)
+            self.steps += 1
 
 
 __all__ = [

@@ -8,6 +8,7 @@ import ast
 import ctypes as C
 import pathlib
 import threading
+import time
 import weakref
 
 import numpy as np
@@ -203,6 +204,31 @@ def test_adamw_tables_and_step_count(backend):
     assert [first[5][i] for i in range(3)] == [g._data.ptr for g in gs]
     assert first[9:] == (0.1, 0.8, 0.95, 1e-6, 0.2, 1, None)
     assert second[9:] == (0.05, 0.8, 0.95, 1e-6, 0.2, 2, scale._data.ptr)
+
+
+def test_adamw_steps_of_two_threads_have_numbers_of_their_own(backend):
+    p, g = _arr(backend, 4), _arr(backend, 4)
+    opt = pb.AdamW([p])
+    steps, both = [], threading.Barrier(2)
+
+    def slow(*args):
+        steps.append(args[14])
+        time.sleep(0.05)
+        return 0
+
+    backend._lib.pb_adamw = slow
+
+    def work():
+        both.wait()
+        for _ in range(3):
+            opt.step([g])
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert steps == [1, 2, 3, 4, 5, 6] and opt.steps == 6
 
 
 def test_adamw_step_on_the_callers_lists(backend):
