@@ -49,16 +49,23 @@ def _context(x, what):
     return backend, dtype, code
 
 
+def _stranger(name, x):
+    return TypeError(f"{name} is no array of the b200 backend: {type(x).__name__}")
+
+
 def _pointer(name, x, shape, dtype, backend):
     """The device pointer of an operand that has to have this shape and dtype
     (None for an operand that is not there)."""
     if x is None:
         return None
-    data = x._data
     # The usual case in three comparisons: a call's time on the host is what its
     # smallest sizes take.
-    if data.backend is backend and x.shape == shape and (x.dtype is dtype or x.dtype == dtype) and data.ptr:
-        return data.ptr
+    try:
+        data = x._data
+        if data.backend is backend and x.shape == shape and (x.dtype is dtype or x.dtype == dtype) and data.ptr:
+            return data.ptr
+    except AttributeError:
+        raise _stranger(name, x) from None
     if data.backend is not backend:
         raise _exc.BackendMismatchError(f"{name} belongs to another backend")
     if tuple(x.shape) != shape:
@@ -74,9 +81,6 @@ def _pointer(name, x, shape, dtype, backend):
 def _output(name, given, shape, dtype, backend, template):
     """``given`` checked, or a new array like ``template``: (array, pointer)."""
     if given is not None:
-        data = given._data
-        if data.backend is backend and given.shape == shape and given.dtype is dtype and data.ptr:
-            return given, data.ptr
         return given, _pointer(name, given, shape, dtype, backend)
     data = backend.empty(shape, dtype)
     return wrap_like(template, data, shape, dtype, backend), data.ptr
@@ -242,8 +246,12 @@ def _table(name, arrays, shapes, dtype, backend):
     """The host table of device pointers of one list, an array for each shape."""
     if len(arrays) != len(shapes):
         raise ValueError(f"{name}: {len(arrays)} arrays for {len(shapes)} parameters")
-    pointers = [x._data.ptr for x, s in zip(arrays, shapes)
-                if x._data.backend is backend and x.dtype is dtype and x.shape == s and x._data.ptr]
+    try:
+        pointers = [x._data.ptr for x, s in zip(arrays, shapes)
+                    if x._data.backend is backend and x.dtype is dtype and x.shape == s and x._data.ptr]
+    except AttributeError:
+        raise _stranger(name, next((x for x in arrays if not hasattr(getattr(x, "_data", None), "backend")),
+                                   arrays)) from None
     if len(pointers) != len(arrays):  # one is not quite so: checked one by one
         pointers = [_pointer(name, x, s, dtype, backend) or 0 for x, s in zip(arrays, shapes)]
     # Through an array of integers: ctypes takes four times as long for each item.
@@ -265,9 +273,12 @@ def _adamw(backend, dtype, code, tables, sizes, grad_scale, lr, betas, eps, weig
     """One step over host tables of parameters, gradients and the two moments."""
     scale = None
     if grad_scale is not None:
-        if prod(grad_scale.shape) != 1:
+        shape = getattr(grad_scale, "shape", None)
+        if shape is None:
+            raise _stranger("grad_scale", grad_scale)
+        if prod(shape) != 1:
             raise ValueError("grad_scale has one element")
-        scale = _pointer("grad_scale", grad_scale, tuple(grad_scale.shape), dtype, backend)
+        scale = _pointer("grad_scale", grad_scale, tuple(shape), dtype, backend)
     with backend._lock:
         backend._require_open()
         status = backend._lib.pb_adamw(backend._ctx, 0, code, len(sizes), *tables, sizes, float(lr), *betas,

@@ -115,6 +115,37 @@ def test_refused_arguments_reach_no_kernel(backend, call, error):
         "pb_recurrence", "pb_recurrence_backward", "pb_group_norm", "pb_group_norm_backward", "pb_adamw")]
 
 
+class _HostArray:
+    """An array of another backend, its data a NumPy array."""
+
+    def __init__(self, *shape):
+        self._data = np.zeros(shape, np.float32)
+        self.shape, self.dtype = shape, self._data.dtype
+
+
+@pytest.mark.parametrize("make", [lambda *s: np.zeros(s, np.float32), _HostArray])
+@pytest.mark.parametrize("call", [
+    lambda a, o: pb.linear_recurrence(o(2, 3, 4), a),
+    lambda a, o: pb.linear_recurrence(a, o(2, 3, 4)),
+    lambda a, o: pb.linear_recurrence(a, a, state=o(2, 4)),
+    lambda a, o: pb.linear_recurrence(a, a, out=o(2, 3, 4)),
+    lambda a, o: pb.linear_recurrence_backward(a, a, a, o(2, 3, 4)),
+    lambda a, o: pb.group_norm(a, 2, o(4)),
+    lambda a, o: pb.group_norm(a, 2, out=(o(2, 3, 4), None, None)),
+    lambda a, o: pb.group_norm_backward(o(2, 3, 4), a, 2, a, a),
+    lambda a, o: pb.AdamW([a, o(4)]),
+    lambda a, o: pb.AdamW([a], exp_avg=[o(2, 3, 4)]),
+    lambda a, o: pb.AdamW([a]).step([o(2, 3, 4)]),
+    lambda a, o: pb.AdamW([a]).step([None]),
+    lambda a, o: pb.AdamW([a]).step([a], grad_scale=o(1)),
+    lambda a, o: pb.AdamW([a]).step([a], grad_scale=0.5),
+    lambda a, o: pb.adamw_step([a], [o(2, 3, 4)], [a], [a], step=1),
+])
+def test_arrays_of_other_kinds_are_a_type_error(backend, call, make):
+    with pytest.raises(TypeError, match="b200 backend"):
+        call(_arr(backend, 2, 3, 4), make)
+
+
 def test_a_closed_backend_is_refused(backend):
     a = _arr(backend, 2, 3, 4)
     opt = pb.AdamW([a])
