@@ -346,6 +346,8 @@ class B200Backend:
                 if dim != 1 and stride != step:
                     raise ValueError("b200 view needs C-contiguous memory")
                 step *= dim
+        if face.get("mask") is not None:
+            raise ValueError("b200 view takes no masked arrays")
         nbytes = prod(shape) * dtype.itemsize
         if nbytes and ptr % 16:
             raise ValueError("b200 view needs 16-byte aligned memory")

@@ -56,6 +56,14 @@ def test_refused_views(host_backend, face, error):
     assert host_backend._lib.calls == []
 
 
+def test_a_masked_array_is_refused(host_backend):
+    """The interface's mask marks values that are not there: they are not to be read as values."""
+    with pytest.raises(ValueError, match="mask"):
+        host_backend.view(_face(mask=_face(typestr="|b1")))
+    assert host_backend._lib.calls == []
+    assert host_backend.view(_face(mask=None)).shape == (3, 5)
+
+
 def test_view_without_the_interface(host_backend):
     with pytest.raises(AttributeError):
         host_backend.view(np.zeros(3, np.float32))
