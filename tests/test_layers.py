@@ -220,6 +220,34 @@ def test_group_norm_views_and_outputs(backend):
     assert backend._lib.calls[-1][1][4:8] == (6, 1, 8, 1)
 
 
+class _FrontArray:
+    """An array of a front end that wraps a backend's buffers, as OpenPacho's does
+    (src/openpacho/_array.py:43-51)."""
+
+    @classmethod
+    def _wrap(cls, data, shape, dtype, backend):
+        x = cls()
+        x._data, x.shape, x.dtype, x._backend = data, shape, dtype, backend
+        return x
+
+
+def test_arrays_of_the_front_end_are_taken_and_returned(backend):
+    def arr(*shape):
+        return _FrontArray._wrap(backend.empty(shape, np.float32), shape, np.dtype(np.float32), backend)
+
+    a, w = arr(2, 3, 4), arr(4)
+    h = pb.linear_recurrence(a, a, state=arr(2, 4), gate="sigmoid")
+    y, mean, rstd = pb.group_norm(h, 2, w, w)
+    grads = pb.group_norm_backward(y, h, 2, mean, rstd, w, w)
+    more = pb.linear_recurrence_backward(a, a, h, grads[0], gate="sigmoid")
+    opt = pb.AdamW([w])
+    opt.step([grads[1]])
+    pb.adamw_step([w], [grads[1]], opt.exp_avg, opt.exp_avg_sq, step=2)
+    shapes = [x.shape for x in (h, y, mean, rstd, *grads, *more, *opt.exp_avg)]
+    assert shapes == [(2, 3, 4)] * 2 + [(2, 2)] * 2 + [(2, 3, 4), (4,), (4,)] + [(2, 3, 4)] * 2 + [(2, 4), (4,)]
+    assert all(type(x) is _FrontArray for x in (h, y, mean, rstd, *grads, *more, *opt.exp_avg))
+
+
 def test_adamw_tables_and_step_count(backend):
     ps = [_arr(backend, 3, 4), _arr(backend, 5), _arr(backend, 0, 2)]
     opt = pb.AdamW(ps, lr=0.1, betas=(0.8, 0.95), eps=1e-6, weight_decay=0.2)
