@@ -264,23 +264,15 @@ struct ChannelResults {
   }
 };
 
-// The first kThreads threads of a block: all of them, or those besides a
-// warp that copies.
-template <bool ALL>
-__device__ __forceinline__ void sync_threads() {
-  if constexpr (ALL) __syncthreads();
-  else asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
-}
-
 // Over the ty rows of threads, in row order: the sums of tx * V channels from c0
-// on, to `out` and to `copy`, which with `more` holds earlier ones that they join.
-template <typename T, int V, bool ALL, typename S>
+// on, to `out` and, where it is another place, to `copy`.
+template <typename T, int V, typename S>
 __device__ __forceinline__ void sum_rows(const NormArgs<T>& p, const S& sums, int64_t c0, int tx, int ty, double2* red,
-                                         double2* out, double2* copy, bool more = false) {
+                                         double2* out, double2* copy) {
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     red[threadIdx.x] = make_double2(sums.s1[i], sums.s2[i]);
-    sync_threads<ALL>();
+    __syncthreads();
     const int64_t c = c0 + (int64_t)threadIdx.x * V + i;
     if ((int)threadIdx.x < tx && c < p.C) {
       double2 t = red[threadIdx.x];
@@ -289,15 +281,9 @@ __device__ __forceinline__ void sum_rows(const NormArgs<T>& p, const S& sums, in
         t.y += red[y * tx + threadIdx.x].y;
       }
       out[c] = t;
-      if (copy && copy != out) {
-        if (more) {
-          t.x += copy[c].x;
-          t.y += copy[c].y;
-        }
-        copy[c] = t;
-      }
+      if (copy && copy != out) copy[c] = t;
     }
-    sync_threads<ALL>();
+    __syncthreads();
   }
 }
 
@@ -344,7 +330,7 @@ __device__ __forceinline__ void sums_item(const NormArgs<T>& p, int64_t unit, in
         sums.add(x, dy);
       }
     }
-    sum_rows<T, V, true>(p, sums, c0, tx, ty, red, out, BWD && p.chan ? p.chan + unit * p.C : nullptr);
+    sum_rows<T, V>(p, sums, c0, tx, ty, red, out, BWD && p.chan ? p.chan + unit * p.C : nullptr);
   }
   sum_groups<T, BWD>(p, out, p.part + unit * p.G);
 }
@@ -367,7 +353,7 @@ __device__ __forceinline__ double2 statistics(const NormArgs<T>& p, int64_t n, i
 
 // The statistics of a sample from its items' group sums.  The threads take
 // (group, every lanes-th item) and meet in shared memory.
-template <typename T, bool BWD, bool ALL>
+template <typename T, bool BWD>
 __device__ __forceinline__ void merge_sample(const NormArgs<T>& p, int64_t n, double2* red) {
   const int wide = p.G < kThreads ? (int)p.G : kThreads, lanes = kThreads / wide;
   const int lg = threadIdx.x % wide, lk = threadIdx.x / wide;
@@ -383,9 +369,9 @@ __device__ __forceinline__ void merge_sample(const NormArgs<T>& p, int64_t n, do
         t.y += v.y;
       }
     }
-    sync_threads<ALL>();
+    __syncthreads();
     red[threadIdx.x] = t;
-    sync_threads<ALL>();
+    __syncthreads();
     if (lk == 0 && g < p.G) {
       for (int k = 1; k < lanes; ++k) {
         t.x += red[k * wide + lg].x;
@@ -460,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) norm_samples_kernel(con
       __syncthreads();
       if (last) {
         __threadfence();
-        merge_sample<T, BWD, true>(p, n, red);
+        merge_sample<T, BWD>(p, n, red);
         __threadfence();
         __syncthreads();
         if (threadIdx.x == 0) {

@@ -87,9 +87,10 @@ struct Device {
   unsigned int* tags = nullptr;
   size_t tags_n = 0;
   unsigned int tag_gen = 0;
-  // Ticket, epoch and flags of the cut recurrence, zeroed when allocated: a flag
-  // is set when it holds the launch's epoch, which the launch itself advances
-  // at its end, so nothing clears it and a replayed graph gets a new one.
+  // Ticket, epoch and flags of the group norm's norm_samples_kernel (its norm_ring_kernel
+  // counts finished blocks there), zeroed when allocated: a flag is set when it holds the
+  // launch's epoch, which the launch itself advances at its end, so nothing clears it
+  // and a replayed graph gets a new one.
   unsigned int* epochs = nullptr;
   size_t epochs_n = 0;
   // Kernel error word in mapped, pinned host memory (no copy needed to read it).
