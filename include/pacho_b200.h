@@ -394,7 +394,9 @@ int pb_reduce(pb_ctx* ctx, int dev, int op, int in_dtype, const void* src, int n
  * an Inf in a or b of its column h is not finite as long as the recurrence
  * written above would not be, but which of the two it is may differ.  A value
  * that leaves the range of the type inside a chunk and that later gates bring
- * back may be there again behind the chunk. */
+ * back may be there again behind the chunk.  A chunk's product of gates is a
+ * float64: one beyond its range gives Inf also where a tiny float64 state or value
+ * would have kept h finite. */
 enum { PB_GATE_LINEAR = 0, PB_GATE_SIGMOID = 1 };
 int pb_recurrence(pb_ctx* ctx, int dev, int dtype, int gate, int64_t outer, int64_t length,
                   int64_t inner, const void* a, const void* b, const void* state, void* h,
@@ -427,8 +429,9 @@ int pb_group_norm(pb_ctx* ctx, int dev, int dtype, int act, int64_t N, int64_t S
 
 /* Gradients of pb_group_norm at the same x, weight and bias, with the mean and
  * rstd it returned.  dx is (N, S, C); dweight and dbias (C values; NULL: not
- * wanted, N == 0: zeros) are sums over N and S, accumulated in float64 in a
- * fixed order.  The derivative of PB_ACT_RELU at 0 is 0. */
+ * wanted, N == 0: zeros) are sums over N and S in a fixed order: up to four terms
+ * at a time in dtype and these in float64, as are the two sums of each group, two
+ * terms at a time.  The derivative of PB_ACT_RELU at 0 is 0. */
 int pb_group_norm_backward(pb_ctx* ctx, int dev, int dtype, int act, int64_t N, int64_t S,
                            int64_t C, int64_t G, const void* dy, const void* x,
                            const void* mean, const void* rstd, const void* weight,

@@ -18,7 +18,7 @@
 // the maps of the segments, and each lane of the second composes those before
 // its own to find its start.  The first pass walks each segment from its end to
 // its start (H += P u, P *= c), so that L2 holds the steps that the second
-// pass reads first.  P and H are float64: a product of thousands of gates
+// pass reads first (1 x 16381 x 1024 float32: 57 of 134 MB).  P and H are float64: a product of thousands of gates
 // neither over- nor underflows where a float32 recurrence does not.  Every
 // composition has a fixed order, so results do not depend on timing.
 //
