@@ -420,7 +420,7 @@ int pb_recurrence_backward(pb_ctx* ctx, int dev, int dtype, int gate, int64_t ou
  * with the variance of the whole set (divided by S * m).  weight and bias
  * (C values; NULL: ones, zeros) are independent of each other.  mean and rstd
  * (N * G values; NULL: not wanted) receive the statistics, which are summed
- * in float64.  PB_ACT_GELU is z * Phi(z) with the normal distribution's Phi.
+ * in float64 (float64 deviations whose squares leave it, about 1e154, give rstd = 0).  PB_ACT_GELU is z * Phi(z) with the normal distribution's Phi.
  * G = 1 with S = 1 is a layer norm of rows of C.  S == 0 or C == 0 is an error. */
 enum { PB_ACT_NONE = 0, PB_ACT_RELU = 1, PB_ACT_SILU = 2, PB_ACT_GELU = 3 };
 int pb_group_norm(pb_ctx* ctx, int dev, int dtype, int act, int64_t N, int64_t S, int64_t C,

@@ -535,6 +535,30 @@ def test_the_kernel_timer_counts_the_sums_of_dweight(b200):
     assert kernels >= whole / 2, (kernels, whole)
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_silu_is_off_by_its_argument_in_roundings(b200, dtype):
+    """As for gelu.  The float32 exponent z log2 e is rounded once (1.3 |z| roundings of
+    the result with the constant's own), and the slope's 1 - s is off by up to four of 1."""
+    b = np.concatenate([np.linspace(-85, 85, 4001), np.linspace(-0.3, 0.3, 800), [0.0]]).astype(dtype)
+    c = b.size
+    rng = np.random.default_rng(6)
+    u = ref.U[np.dtype(dtype)]
+    z = b.astype(np.float64)
+    x = rng.standard_normal((1, 1, c)).astype(dtype)
+    y, _, _ = pb.group_norm(up(b200, x), 1, up(b200, np.zeros(c, dtype)), up(b200, b), activation="silu")
+    want = ref.activate(z, "silu")
+    k = u * (ref.ACT + 1.3 * np.abs(z))
+    close(y.numpy()[0, 0], want, k * np.abs(want), dtype, "silu")
+    stats = [up(b200, v) for v in (np.zeros((1, 1), dtype), np.ones((1, 1), dtype))]
+    dy = rng.standard_normal((1, 1, c)).astype(dtype)
+    _, _, dbias = pb.group_norm_backward(up(b200, dy), up(b200, x), 1, *stats, up(b200, np.zeros(c, dtype)), up(b200, b),
+                                         activation="silu")
+    s, rest = ref.sigmoid(z)
+    g = np.abs(dy[0, 0].astype(np.float64))
+    close(dbias.numpy(), dy[0, 0] * ref.slope(z, "silu"), g * (k * (s + np.abs(s * z) * rest) + 4 * u * np.abs(s * z)),
+          dtype, "slope")
+
+
 # (N, S, C, G) of the ring's further ways: sums of more blocks and groups than each
 # block adds up for itself (8192, or 512 groups), with packs and with single values; and
 # several rounds of samples, the per-block sums of dweight and dbias carried on.
