@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, BWD ? 2 : 3) norm_samples_kernel(con
 // the 16-byte boundaries around them, the last values of the array apart; a thread's
 // channels lie tx apart, so that lanes move neighbours one value at a time.
 // 8 x 4096 x 319 float32 forward 33 us (plain loads of norm_samples_kernel: 69; 320
-// channels: 31), backward 63 (124; 54); 6 x 3001 x 1107 forward 64 (125).
+// channels: 31), backward 60 (124; 55); 6 x 3001 x 1107 forward 64 (125).
 constexpr int kRingThreads = 480;  // and a warp that copies: 16 warps, 128 registers each thread
 constexpr int kRingWarps = kRingThreads / 32;
 constexpr int kRing = 8;
